@@ -16,6 +16,7 @@ HOST_LIB_PATH = os.path.join(HERE, "lib", "libnts_amd.so")
 
 X_TRANS, X_NOTRANS = 0, 1           # MATRIX_TRANS_TYPE, source/tensor/XDataType.h:36
 X_INT, X_FLOAT, X_FLOAT16 = 0, 2, 3  # TENSOR_DATA_TYPE, source/tensor/XDataType.h:33
+ROTATE_HALVES, ROTATE_PAIRS = 0, 1
 BIAS_NONE, BIAS_COL, BIAS_ROW = 0, 1, 2
 ACT_NONE, ACT_RECTIFY = 0, 1
 
@@ -39,9 +40,26 @@ EXPORTS = (
     "ntsamd_matrix_mul_static",
 )
 
+# declared in include/ntsamd_cache.h
+CACHE_EXPORTS = (
+    "ntsamd_cache_append",
+    "ntsamd_attention_cached",
+    "ntsamd_attention_prefix",
+)
+
 
 class NtsAmdError(RuntimeError):
     pass
+
+
+class _Cache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dataType", C.c_int), ("pages", C.c_int), ("pageSize", C.c_int),
+                ("heads", C.c_int), ("dh", C.c_int), ("strides", C.c_longlong * 6)]
+
+
+class _CacheBatch(C.Structure):
+    _fields_ = [("lengths", C.c_void_p), ("starts", C.c_void_p), ("pageTable", C.c_void_p), ("sequences", C.c_int),
+                ("tablePages", C.c_int), ("tokens", C.c_int), ("maxNew", C.c_int), ("maxLength", C.c_int)]
 
 
 def build(jobs=8):
@@ -82,13 +100,16 @@ def load():
     L.ntsamd_convert_data_type.argtypes = [ci, vp, vp, ci, vp, ci, ll]
     L.ntsamd_release_workspaces.argtypes = [ci]
     L.ntsamd_matrix_mul_static.argtypes = L.ntsamd_matrix_mul.argtypes + [ci]
+    L.ntsamd_cache_append.argtypes = [ci, vp, vp, vp, vp, vp, vp, vp, ci, vp, vp, ci, ci, ci]
+    L.ntsamd_attention_cached.argtypes = [ci, vp, vp, vp, vp, vp, ci, vp, cf, ci]
+    L.ntsamd_attention_prefix.argtypes = L.ntsamd_attention_cached.argtypes + [ci]
     # measurement knobs: exported, but no part of the interface include/ntsamd_gemm.h documents
     L.ntsamd_tuning_set.argtypes = [C.c_char_p, ci]
     L.ntsamd_tuning_set.restype = ci
     L.ntsamd_last_plan.restype = C.c_char_p
     L.ntsamd_plan_only.argtypes = [ci]
     L.ntsamd_plan_only.restype = None
-    for name in EXPORTS[2:]:
+    for name in EXPORTS[2:] + CACHE_EXPORTS:
         getattr(L, name).restype = ci
     _lib = L
     return L
@@ -325,3 +346,99 @@ def convert_data_type(s, t):
                                          t.data_ptr(), _dtype_code(t), s.numel())
     _check(rc)
     return t
+
+
+class KVCache:
+    """A cache of keys and values on pages (include/ntsamd_cache.h) over two tensors of the caller, float32 or float16,
+    [pages][positions of a page][heads][dh]; any strides with contiguous columns, so a pool stored
+    [pages][heads][positions][dh] is passed as its transpose(1, 2). Keep it as long as the cache lives."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise NtsAmdError("Unmatched tensors in the cache!")
+        if k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
+            raise NtsAmdError("the columns of the cache must be contiguous")
+        self.k, self.v = k, v
+        self.dtype, self.device, self.heads, self.dh = k.dtype, k.device, int(k.shape[2]), int(k.shape[3])
+        self._c = _Cache(k.data_ptr(), v.data_ptr(), _dtype_code(k), k.shape[0], k.shape[1], k.shape[2], k.shape[3],
+                         (C.c_longlong * 6)(*k.stride()[:3], *v.stride()[:3]))
+        self._ref = C.addressof(self._c)
+
+
+class CacheBatch:
+    """The sequences of one step: lengths, the new positions included; page_table [sequences][pages]; starts
+    [sequences + 1], the rows of q, k, v and out where each sequence's new tokens begin, or None if every sequence has
+    max_new of them. int32 device tensors, which may be refilled between calls within max_new new tokens and
+    max_length positions a sequence (default: what page_table holds)."""
+
+    def __init__(self, lengths, page_table, starts=None, tokens=None, max_new=1, max_length=0):
+        import torch
+        for t in (lengths, page_table, starts):
+            if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.device != lengths.device):
+                raise NtsAmdError("lengths, page table and starts must be dense int32 tensors on one device")
+        n = int(lengths.numel())
+        if page_table.dim() != 2 or page_table.shape[0] != n or (starts is not None and starts.numel() != n + 1):
+            raise NtsAmdError("Unmatched tensors in the batch!")
+        self.tensors = (lengths, page_table, starts)
+        self.tokens = n * max_new if tokens is None else int(tokens)
+        self.device = lengths.device
+        self._c = _CacheBatch(lengths.data_ptr(), starts.data_ptr() if starts is not None else None, page_table.data_ptr(),
+                              n, page_table.shape[1], self.tokens, max_new, max_length)
+        self._ref = C.addressof(self._c)
+
+
+def _rows(t, cache, batch, heads):
+    """Token and head strides of a [tokens][heads][dh] tensor of the cache's type, on its device."""
+    if t.dim() != 3 or t.dtype != cache.dtype or t.device != cache.device or batch.device != cache.device:
+        raise NtsAmdError("rows of the cache's data type and device, [tokens][heads][dh], are wanted")
+    n, h, d = t.shape
+    s = t.stride()
+    if n != batch.tokens or h != heads or d != cache.dh or (s[2] != 1 and d > 1):
+        raise NtsAmdError("Unmatched tensors: %s for %d tokens, %d heads of %d contiguous columns"
+                          % (tuple(t.shape), batch.tokens, heads, cache.dh))
+    return s[0], s[1]
+
+
+def cache_append(cache, batch, k, v, rotation=None, pairs=False, q=None, q_out=None):
+    """The new tokens' keys and values ([tokens][heads][dh], any strides) to their places in the cache; keys, and
+    queries to q_out (which may be q), turned by rotation: float [positions][columns / 2][2] of cosine and sine.
+    pairs: neighbouring columns are turned together, otherwise column j and j + columns / 2."""
+    ks, vs = _rows(k, cache, batch, cache.heads), _rows(v, cache, batch, cache.heads)
+    qs = os_ = (0, 0)
+    heads = 0
+    if q is not None:
+        heads = int(q.shape[1])
+        qs, os_ = _rows(q, cache, batch, heads), _rows(q_out, cache, batch, heads)
+    positions = rotated = 0
+    if rotation is not None:
+        if rotation.dim() != 3 or rotation.shape[2] != 2 or not rotation.is_contiguous() or _dtype_code(rotation) != X_FLOAT \
+                or rotation.device != cache.device:
+            raise NtsAmdError("rotation must be a dense float [positions][columns / 2][2] tensor")
+        positions, rotated = int(rotation.shape[0]), 2 * int(rotation.shape[1])
+    rc = load().ntsamd_cache_append(cache.device.index, _stream_ptr(k), cache._ref, batch._ref, k.data_ptr(), v.data_ptr(),
+                                    q.data_ptr() if q is not None else None, q_out.data_ptr() if q is not None else None, heads,
+                                    (C.c_longlong * 8)(*ks, *vs, *qs, *os_),
+                                    rotation.data_ptr() if rotation is not None else None, positions, rotated,
+                                    ROTATE_PAIRS if pairs else ROTATE_HALVES)
+    _check(rc)
+    return q_out
+
+
+def attention_cached(cache, batch, q, out, scale, causal=True):
+    """out = softmax(scale q k^T) v over each sequence's positions in the cache; q and out [tokens][heads][dh], heads a
+    multiple of the cache's. causal: a token sees its own position and those before it, otherwise all of them."""
+    heads = int(q.shape[1])
+    strides = (C.c_longlong * 4)(*_rows(q, cache, batch, heads), *_rows(out, cache, batch, heads))
+    _check(load().ntsamd_attention_cached(cache.device.index, _stream_ptr(q), cache._ref, batch._ref, q.data_ptr(), out.data_ptr(),
+                                          heads, strides, scale, 1 if causal else 0))
+    return out
+
+
+def attention_prefix(cache, batch, q, out, scale, prefix, causal=True):
+    """attention_cached for sequences whose first `prefix` positions hold the same keys and values, which are read through
+    the first row of the page table, once for all sequences."""
+    heads = int(q.shape[1])
+    strides = (C.c_longlong * 4)(*_rows(q, cache, batch, heads), *_rows(out, cache, batch, heads))
+    _check(load().ntsamd_attention_prefix(cache.device.index, _stream_ptr(q), cache._ref, batch._ref, q.data_ptr(), out.data_ptr(),
+                                          heads, strides, scale, 1 if causal else 0, prefix))
+    return out

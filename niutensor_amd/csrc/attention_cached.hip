@@ -1,0 +1,520 @@
+/*
+ * Attention of new tokens over a cache on pages (ntsamd_attention_cached, ntsamd_attention_prefix;
+ * include/ntsamd_cache.h):  out[t][h] = sum_j p_j v_j,  p = softmax_j(scale <q[t][h], k_j>),  j over the positions that t sees.
+ *
+ * A step of one token per sequence reads every key and value once and computes 4 R operations per element (R query
+ * heads share a key head): bound by memory by far, so the plan is to keep loads in flight and to spread the keys evenly.
+ *
+ * A workgroup takes up to 16 QR query rows (tokens x the query heads of one key head) of one sequence and a range of
+ * its keys; its four waves take units of UK keys (32 half, 16 float: 8 KB of k and 8 KB of v at 128 columns) in turn, each
+ * with a running softmax of its own, and nothing is shared until the range is done. Both products run on MFMAs, transposed
+ * (as in attention_f32.hip), so that the probabilities pass from accumulator to operand inside a lane:
+ *   S^T = K Q^T   lane (m, g) = (l % 16, l / 16) feeds columns of key m and of query m, and receives the scores of query m
+ *                 against keys 16 j + 4 g + r, r = 0..3;
+ *   O^T = V^T P^T lane (m, g) feeds the probabilities it holds, and of V its keys in VC neighbouring columns, VC m ...: the
+ *                 rows of V^T may stand for any columns, so MFMA c of a set takes column VC m + c, and a lane's
+ *                 16-byte loads of VC columns of its keys are what the set needs. In half, where a lane feeds eight keys
+ *                 of one column, the 8 x VC piece it loaded is transposed by byte permutes within the lane.
+ * So k and v go from memory to registers, each element once, without LDS; the next unit is in flight while one is
+ * computed, the page numbers of the one after it are looked up by the lanes, one key each, and handed round.
+ * Addresses of positions that a range does not have, and of columns past dh, point at a row of zeros: nothing behind a
+ * sequence's end is ever read, let alone multiplied.
+ *
+ * The four waves' results meet in LDS. Where a range is not all of a sequence's keys, the result is a partial one
+ * (unnormalised row, maximum, sum), and a second kernel joins them in the order of the keys.
+ */
+#include "gemm_common.h"
+#include "gemm_f16.h"       /* half_t */
+#include "attention.h"
+#include "attention_cached.h"
+
+namespace ntsamd {
+
+namespace {
+
+__device__ const float zero_row[4] = {0.f, 0.f, 0.f, 0.f};
+
+template <typename T, int DHM> struct Unit;
+template <int DHM> struct Unit<half_t, DHM> {
+    static constexpr int UK = 32, NJ = 2;               /* keys, blocks of 16 of them */
+    static constexpr int NT = DHM / 32;                 /* 16-byte pieces of a key row per lane */
+    static constexpr int NV = 8;                        /* keys whose values a lane loads */
+    static constexpr int VC = DHM / 16, NH = 1;         /* neighbouring columns of them, sets of such columns */
+    typedef f16x8 KPiece;
+    typedef half_t VPiece __attribute__((ext_vector_type(VC)));
+};
+template <int DHM> struct Unit<float, DHM> {
+    static constexpr int UK = 16, NJ = 1;
+    static constexpr int NT = DHM / 16;
+    static constexpr int NV = 4;
+    static constexpr int VC = DHM >= 64 ? 4 : DHM / 16, NH = DHM / 16 / VC;
+    typedef f32x4 KPiece;
+    typedef float VPiece __attribute__((ext_vector_type(VC)));
+};
+
+template <typename T, int DHM> struct UnitData {
+    typename Unit<T, DHM>::KPiece k[Unit<T, DHM>::NJ][Unit<T, DHM>::NT];
+    typename Unit<T, DHM>::VPiece v[Unit<T, DHM>::NV][Unit<T, DHM>::NH];
+    unsigned there;                                     /* which of its keys exist */
+};
+
+__device__ __forceinline__ long long lane_of(long long x, int source)
+{
+    const int lo = __shfl((int)x, source), hi = __shfl((int)(x >> 32), source);
+    return ((long long)hi << 32) | (unsigned)lo;
+}
+
+/* ND columns from `col` on, those below dh, times f */
+template <typename T, int ND>
+__device__ __forceinline__ void store_columns(T * row, int col, int dh, const float (&x)[ND], float f)
+{
+    constexpr int W = ND < 16 / (int)sizeof(T) ? ND : 16 / (int)sizeof(T);      /* dh is a multiple of 16 / sizeof(T) */
+    typedef T vec __attribute__((ext_vector_type(W)));
+#pragma unroll
+    for (int at = 0; at < ND; at += W)
+        if (col + at < dh) {
+            vec v;
+#pragma unroll
+            for (int e = 0; e < W; e++)
+                v[e] = (T)(x[at + e] * f);
+            *reinterpret_cast<vec *>(row + col + at) = v;
+        }
+}
+
+/* a range of the keys of one tile of rows */
+struct Segment {
+    CacheSequence s;
+    int seq, head;                      /* table row, key head */
+    int row0, rows;                     /* first row of the tile, rows the sequence has */
+    int u0, u1;                         /* units, from p.first on */
+    int slot;                           /* where the partial result goes, -1: the result goes to out */
+};
+
+/* The sequences of this lane's rows in a launch over the shared prefix, whose rows are the tokens of all sequences: the
+   last one that starts at or before the row's token, searched for in LDS. */
+template <int QR>
+__device__ __forceinline__ void row_sequences(const CachedParams & p, const Segment & sg, CachedShared & sh, int (&seq)[QR])
+{
+    constexpr int N = 4096;
+    static_assert(N * sizeof(int) <= sizeof(sh.acc), "");
+    int * from = reinterpret_cast<int *>(&sh.acc[0][0][0]);
+    const int m = threadIdx.x & 15;
+    int tok[QR], count[QR];
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const int row = sg.row0 + 16 * q + m;
+        tok[q] = sg.s.start + (row < sg.rows ? divided(row, p.perDiv) : 0);
+        count[q] = 0;
+    }
+    for (int i0 = 0; i0 < p.seqs; i0 += N) {
+        const int n = min(N, p.seqs - i0);
+        for (int i = threadIdx.x; i < n; i += 256)
+            from[i] = p.c.starts[p.seq0 + i0 + i];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < QR; q++) {
+            int lo = 0, hi = n;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (from[mid] <= tok[q])
+                    lo = mid + 1;
+                else
+                    hi = mid;
+            }
+            count[q] += lo;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < QR; q++)
+        seq[q] = p.seq0 + max(count[q] - 1, 0);
+}
+
+template <typename T, int DHM, int QR>
+__device__ __forceinline__ void attend(const CachedParams & p, const Segment & sg, CachedShared & sh)
+{
+    typedef Unit<T, DHM> U;
+    constexpr int ND = DHM / 16;
+    constexpr float LOG2E = 1.4426950408889634f;
+    constexpr unsigned ALL = U::UK == 32 ? 0xffffffffu : 0xffffu;
+    const CacheParams & c = p.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    const int dh = c.dh;
+
+    /* ---- this lane's query rows: positions each sees, fragments ---- */
+    int seen[QR] = {};
+    typename U::KPiece qf[QR][U::NT];
+    if (p.prefix > 0 && c.starts)
+        row_sequences<QR>(p, sg, sh, seen);             /* for now: the sequence of each row */
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const int row = sg.row0 + 16 * q + m;
+        const bool there = row < sg.rows;
+        const int t = there ? divided(row, p.perDiv) : 0;
+        const int h = sg.head * p.per + (there ? row - t * p.per : 0);
+        if (!there)
+            seen[q] = 0x7fffffff;                       /* padding: computed with, never stored */
+        else if (p.prefix > 0) {
+            const int seq = c.starts ? seen[q] : p.seq0 + t / c.maxNew;
+            const CacheSequence s = cache_sequence(c, seq);
+            seen[q] = min(p.causal ? s.length - s.fresh + (sg.s.start + t - s.start) + 1 : s.length, p.prefix);
+        }
+        else
+            seen[q] = p.causal ? sg.s.length - sg.s.fresh + t + 1 : sg.s.length;
+        const T * qr = static_cast<const T *>(p.q) + (long long)(sg.s.start + t) * p.qT + h * p.qH;
+#pragma unroll
+        for (int t4 = 0; t4 < U::NT; t4++) {
+            constexpr int W = sizeof(typename U::KPiece) / sizeof(T);
+            const int col = 4 * W * t4 + W * g;
+            typename U::KPiece z = {};
+            qf[q][t4] = there && col < dh ? *reinterpret_cast<const typename U::KPiece *>(qr + col) : z;
+        }
+    }
+    int seenMin = seen[0], seenMax = 0;
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        seenMin = min(seenMin, seen[q]);
+        seenMax = max(seenMax, seen[q] == 0x7fffffff ? 0 : seen[q]);
+    }
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) {
+        seenMin = min(seenMin, __shfl_xor(seenMin, d));
+        seenMax = max(seenMax, __shfl_xor(seenMax, d));
+    }
+    seenMin = __builtin_amdgcn_readfirstlane(seenMin);
+    seenMax = __builtin_amdgcn_readfirstlane(seenMax);
+
+    /* ---- loading a unit ---- */
+    const int * table = c.table + (long long)sg.seq * c.tablePages;
+    const char * kBase = reinterpret_cast<const char *>(static_cast<const T *>(c.k) + sg.head * c.kH);
+    const char * vBase = reinterpret_cast<const char *>(static_cast<const T *>(c.v) + sg.head * c.vH);
+    const char * zero = reinterpret_cast<const char *>(zero_row);
+    const int myKey = lane & (U::UK - 1);
+    auto page_of = [&](int u) {
+        const int key = p.first + u * U::UK + myKey;
+        return u < sg.u1 && key < seenMax ? table[divided(key, c.pageSize)] : -1;
+    };
+    auto load = [&](int u, int page, UnitData<T, DHM> & d) {
+        const int key = p.first + u * U::UK + myKey;
+        const bool valid = page >= 0 && page < c.pages;
+        const int r = key - divided(key, c.pageSize) * (int)c.pageSize.d;
+        const long long kOff = valid ? (page * c.kP + r * c.kR) * (long long)sizeof(T) : -1;
+        const long long vOff = valid ? (page * c.vP + r * c.vR) * (long long)sizeof(T) : -1;
+        d.there = (unsigned)__ballot(valid) & ALL;
+#pragma unroll
+        for (int j = 0; j < U::NJ; j++) {
+            const long long off = lane_of(kOff, 16 * j + m);
+            const char * row = kBase + off;
+#pragma unroll
+            for (int t = 0; t < U::NT; t++) {
+                const int col = (64 * t + 16 * g) / (int)sizeof(T);
+                d.k[j][t] = *reinterpret_cast<const typename U::KPiece *>(off >= 0 && col < dh ? row + 64 * t + 16 * g : zero);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < U::NV; e++) {
+            const long long off = lane_of(vOff, 16 * (e >> 2) + 4 * g + (e & 3));
+            const char * row = vBase + off;
+#pragma unroll
+            for (int h = 0; h < U::NH; h++) {
+                const int col = U::VC * (16 * h + m);
+                d.v[e][h] = *reinterpret_cast<const typename U::VPiece *>(off >= 0 && col < dh ? row + col * (int)sizeof(T) : zero);
+            }
+        }
+    };
+
+    f32x4 accO[QR][ND];
+    float rowMax[QR], rowSum[QR];
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            accO[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        rowMax[q] = -INFINITY;
+        rowSum[q] = 0.f;
+    }
+    const float scale2 = p.scale * LOG2E;
+
+    UnitData<T, DHM> next;
+    int u = sg.u0 + wave;
+    int page = page_of(u);
+    if (u < sg.u1)
+        load(u, page, next);
+    page = page_of(u + 4);
+    for (; u < sg.u1; u += 4) {
+        const UnitData<T, DHM> d = next;
+        if (u + 4 < sg.u1)
+            load(u + 4, page, next);
+        page = page_of(u + 8);
+
+        /* ---- S^T = K Q^T ---- */
+        f32x4 s[QR][U::NJ];
+#pragma unroll
+        for (int q = 0; q < QR; q++)
+#pragma unroll
+            for (int j = 0; j < U::NJ; j++)
+                s[q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < U::NT; t++)
+#pragma unroll
+            for (int j = 0; j < U::NJ; j++)
+#pragma unroll
+                for (int q = 0; q < QR; q++) {
+                    if constexpr (sizeof(T) == 2)
+                        s[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d.k[j][t], qf[q][t], s[q][j], 0, 0, 0);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            s[q][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(d.k[j][t][e], qf[q][t][e], s[q][j], 0, 0, 0);
+                    }
+                }
+
+        const int key0 = p.first + u * U::UK;
+        const bool cut = d.there != ALL || key0 + U::UK > seenMin;
+        T pr[QR][U::NJ][4];                             /* the probabilities as the second product's operand */
+#pragma unroll
+        for (int q = 0; q < QR; q++) {
+#pragma unroll
+            for (int j = 0; j < U::NJ; j++)
+                s[q][j] *= scale2;
+            if (cut) {
+#pragma unroll
+                for (int j = 0; j < U::NJ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int at = 16 * j + 4 * g + r;
+                        if (!((d.there >> at) & 1) || key0 + at >= seen[q])
+                            s[q][j][r] = -INFINITY;
+                    }
+            }
+            float mx = s[q][0][0];
+#pragma unroll
+            for (int j = 0; j < U::NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    mx = fmaxf(mx, s[q][j][r]);
+            const float newMax = fmaxf(rowMax[q], lane_groups_max(mx));
+            const float shift = newMax == -INFINITY ? 0.f : newMax;
+            const float corr = __builtin_amdgcn_exp2f(rowMax[q] - shift);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < U::NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float e = __builtin_amdgcn_exp2f(s[q][j][r] - shift);
+                    sum += e;
+                    pr[q][j][r] = (T)e;
+                }
+            rowSum[q] = rowSum[q] * corr + sum;         /* this lane's keys only: the lanes of a row meet at the end */
+            rowMax[q] = newMax;
+#pragma unroll
+            for (int e = 0; e < ND; e++)
+                accO[q][e] *= corr;
+        }
+
+        /* ---- O^T += V^T P^T ---- */
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int v = 0; v < U::VC; v++) {
+                f16x8 a;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    a[e] = d.v[e][0][v];
+#pragma unroll
+                for (int q = 0; q < QR; q++) {
+                    const f16x8 b = {pr[q][0][0], pr[q][0][1], pr[q][0][2], pr[q][0][3],
+                                     pr[q][1][0], pr[q][1][1], pr[q][1][2], pr[q][1][3]};
+                    accO[q][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, accO[q][v], 0, 0, 0);
+                }
+            }
+        }
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int h = 0; h < U::NH; h++)
+#pragma unroll
+                    for (int v = 0; v < U::VC; v++)
+#pragma unroll
+                        for (int q = 0; q < QR; q++)
+                            accO[q][h * U::VC + v] =
+                                __builtin_amdgcn_mfma_f32_16x16x4f32(d.v[e][h][v], pr[q][0][e], accO[q][h * U::VC + v], 0, 0, 0);
+        }
+    }
+
+    /* ---- the four waves' results, 16 rows at a time. Register r of MFMA v of set h holds column VC (16 h + 4 g + r) + v of
+       the lane's row ---- */
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const float sum = lane_groups_sum(rowSum[q]);
+        if (g == 0) {
+            sh.stat[wave][m][0] = rowMax[q];
+            sh.stat[wave][m][1] = sum;
+        }
+#pragma unroll
+        for (int h = 0; h < U::NH; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int v = 0; v < U::VC; v++)
+                    sh.acc[wave][m][U::VC * (16 * h + 4 * g + r) + v] = accO[q][h * U::VC + v][r];
+        __syncthreads();
+        const int mine = tid >> 4, col = (tid & 15) * ND, row = sg.row0 + 16 * q + mine;
+        if (row < sg.rows) {
+            float mx = sh.stat[0][mine][0];
+#pragma unroll
+            for (int w = 1; w < 4; w++)
+                mx = fmaxf(mx, sh.stat[w][mine][0]);
+            const float shift = mx == -INFINITY ? 0.f : mx;
+            float total = 0.f, o[ND];
+#pragma unroll
+            for (int e = 0; e < ND; e++)
+                o[e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float f = __builtin_amdgcn_exp2f(sh.stat[w][mine][0] - shift);
+                total += f * sh.stat[w][mine][1];
+#pragma unroll
+                for (int e = 0; e < ND; e++)
+                    o[e] += f * sh.acc[w][mine][col + e];
+            }
+            if (sg.slot < 0) {
+                const int t = divided(row, p.perDiv);
+                T * out = static_cast<T *>(p.out) + (long long)(sg.s.start + t) * p.oT + (sg.head * p.per + row - t * p.per) * p.oH;
+                store_columns<T, ND>(out, col, dh, o, total == 0.f ? 0.f : 1.f / total);
+            }
+            else {
+                const long long at = (long long)sg.slot * p.rows + (row - sg.row0);
+                store_columns<float, ND>(p.acc + at * dh, col, dh, o, 1.f);
+                if ((tid & 15) == 0) {
+                    p.stat[2 * at] = mx;
+                    p.stat[2 * at + 1] = total;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int DHM, int QR>
+__global__ void __launch_bounds__(256, QR == 1 ? 2 : 1)
+attention_cached_kernel(const CachedParams p)
+{
+    constexpr int UK = Unit<T, DHM>::UK, TR = 16 * QR;
+    __shared__ CachedShared sh;
+    const int id = (int)blockIdx.x;
+    Segment sg;
+    if (p.mode == CACHED_WHOLE) {
+        const int i = id / p.c.kvHeads;
+        sg.head = id - i * p.c.kvHeads;
+        sg.seq = p.seq0 + i;
+        sg.s = cache_sequence(p.c, sg.seq);
+        sg.row0 = 0;
+        sg.rows = sg.s.fresh * p.per;
+        sg.u0 = 0;
+        sg.u1 = (max(sg.s.length - p.first, 0) + UK - 1) / UK;
+        sg.slot = p.acc ? id : -1;
+        if (sg.rows > 0)
+            attend<T, DHM, QR>(p, sg, sh);
+    }
+    else if (p.mode == CACHED_FLAT) {
+        const FlatPlan f = flat_plan<UK>(p, sh);
+        if (id >= f.groups)
+            return;
+        const long long begin = f.start(id), end = f.start(id + 1);
+        long long before;
+        int i = find_sequence(f.scan, begin, before, sh,
+                              [&](int n) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + n)) * p.c.kvHeads; });
+        for (long long at = begin; at < end;) {
+            sg.seq = p.seq0 + i;
+            sg.s = cache_sequence(p.c, sg.seq);
+            const int units = units_of<UK>(p, sg.s);
+            for (; at < end && at < before + (long long)units * p.c.kvHeads;) {
+                const long long in = at - before;
+                sg.head = (int)(in / units);
+                sg.u0 = (int)(in - (long long)sg.head * units);
+                sg.u1 = (int)min((long long)units, sg.u0 + (end - at));
+                sg.row0 = 0;
+                sg.rows = sg.s.fresh * p.per;
+                if (sg.u0 == 0 && sg.u1 == units)
+                    sg.slot = p.first > 0 ? 2 * p.groups + i * p.c.kvHeads + sg.head : -1;
+                else
+                    sg.slot = 2 * id + (at == begin ? 0 : 1);
+                attend<T, DHM, QR>(p, sg, sh);
+                at += sg.u1 - sg.u0;
+            }
+            before += (long long)units * p.c.kvHeads;
+            i++;
+        }
+    }
+    else {
+        /* the last tiles of a sequence see the most keys: first */
+        const int perTile = p.c.kvHeads * p.groups;
+        int tile = p.tiles - 1 - id / perTile;
+        const int rest = id % perTile, piece = rest / p.c.kvHeads;
+        sg.head = rest - piece * p.c.kvHeads;
+        const int slot = (tile * p.c.kvHeads + sg.head) * p.groups + piece;
+        if (p.prefix > 0) {
+            sg.s.start = cache_sequence(p.c, p.seq0).start;
+            sg.s.fresh = prefix_tokens(p, sg.s.start);
+            sg.s.length = p.prefix;
+            sg.seq = 0;
+        }
+        else {
+            const auto tiles = [&](int n) { return (long long)((cache_sequence(p.c, p.seq0 + n).fresh * p.per + TR - 1) / TR); };
+            const SequenceScan scan = scan_sequences(p.seqs, sh, tiles);
+            long long before;
+            const int i = find_sequence(scan, tile, before, sh, tiles);
+            if (i < 0)
+                return;
+            tile -= (int)before;
+            sg.seq = p.seq0 + i;
+            sg.s = cache_sequence(p.c, sg.seq);
+        }
+        sg.rows = sg.s.fresh * p.per;
+        sg.row0 = tile * TR;
+        if (sg.row0 >= sg.rows)
+            return;
+        int keys = sg.s.length;
+        if (p.causal && p.prefix == 0)
+            keys -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
+        const int units = (max(keys - p.first, 0) + UK - 1) / UK;
+        sg.u0 = (int)((long long)units * piece / p.groups);
+        sg.u1 = (int)((long long)units * (piece + 1) / p.groups);
+        sg.slot = p.acc ? slot : -1;
+        attend<T, DHM, QR>(p, sg, sh);
+    }
+}
+
+template <typename T, int DHM>
+int launch_dhm(const CachedParams & p, int qr, int blocks, hipStream_t stream)
+{
+    const dim3 grid((unsigned)blocks), block(256);
+    if (qr == 1)
+        hipLaunchKernelGGL((attention_cached_kernel<T, DHM, 1>), grid, block, 0, stream, p);
+    else if (qr == 2)
+        hipLaunchKernelGGL((attention_cached_kernel<T, DHM, 2>), grid, block, 0, stream, p);
+    else
+        hipLaunchKernelGGL((attention_cached_kernel<T, DHM, 4>), grid, block, 0, stream, p);
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int launch_type(const CachedParams & p, int qr, int blocks, hipStream_t stream)
+{
+    if (p.c.dh <= 32)
+        return launch_dhm<T, 32>(p, qr, blocks, stream);
+    if (p.c.dh <= 64)
+        return launch_dhm<T, 64>(p, qr, blocks, stream);
+    return launch_dhm<T, 128>(p, qr, blocks, stream);
+}
+
+}  // namespace
+
+int launch_attention_cached(const CachedParams & p, bool half, int qr, int blocks, hipStream_t stream)
+{
+    return half ? launch_type<half_t>(p, qr, blocks, stream) : launch_type<float>(p, qr, blocks, stream);
+}
+
+}  // namespace ntsamd

@@ -1,12 +1,14 @@
 /*
  * C ABI of the gfx950 matrix-multiplication library (declared in
- * include/ntsamd_gemm.h): argument checking, device handling and the choice
+ * include/ntsamd_gemm.h and include/ntsamd_cache.h): argument checking, device handling and the choice
  * of kernel. Takes the place of source/tensor/core/arithmetic/XTensorBLAS.cu
  * in the reference.
  */
 #include "../../include/ntsamd_gemm.h"
+#include "../../include/ntsamd_cache.h"
 #include "gemm_common.h"
 #include "attention.h"
+#include "attention_cached.h"
 
 #include <atomic>
 #include <map>
@@ -937,6 +939,309 @@ int check_pointers(const void * a, const void * b, const void * c)
     return NTSAMD_OK;
 }
 
+/* ---- the cache of keys and values on pages (include/ntsamd_cache.h) ---------------------------------------- */
+
+/* whether two of the rows of `width` elements that n counted strides lead to share an element: taken from the shortest
+   stride up, each must step over everything the shorter ones span */
+bool rows_overlap(const long long * strides, const long long * counts, int n, long long width)
+{
+    long long st[3], ct[3];
+    for (int i = 0; i < n; i++) {
+        int at = i;
+        for (; at > 0 && st[at - 1] > strides[i]; at--) {
+            st[at] = st[at - 1];
+            ct[at] = ct[at - 1];
+        }
+        st[at] = strides[i];
+        ct[at] = counts[i];
+    }
+    long long span = width;
+    for (int i = 0; i < n; i++) {
+        if (ct[i] <= 1)
+            continue;
+        if (st[i] < span)
+            return true;
+        span += (ct[i] - 1) * st[i];
+    }
+    return false;
+}
+
+/* What the entry points of the cache check alike. `empty` is set where there is nothing to do. */
+int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, CacheParams & c, bool & empty)
+{
+    empty = false;
+    if (!cache || !batch)
+        return fail(NTSAMD_ERR_ARGUMENT, "Empty input tensors!");
+    if (cache->dataType != NTSAMD_X_FLOAT && cache->dataType != NTSAMD_X_FLOAT16)
+        return fail(NTSAMD_ERR_DATATYPE, "Unsupported data type!");
+    if (cache->pages < 0 || cache->heads < 0 || cache->dh < 0 || batch->sequences < 0 || batch->tablePages < 0 ||
+        batch->tokens < 0 || batch->maxNew < 0 || batch->maxLength < 0)
+        return fail(NTSAMD_ERR_ARGUMENT, "negative tensor size");
+    if (cache->pageSize < 1)
+        return fail(NTSAMD_ERR_ARGUMENT, "pages of %d positions", cache->pageSize);
+    if (batch->sequences == 0 || batch->tokens == 0 || batch->maxNew == 0 || cache->heads == 0 || cache->dh == 0) {
+        empty = true;
+        return NTSAMD_OK;
+    }
+    const int vec = cache->dataType == NTSAMD_X_FLOAT ? 4 : 8;
+    if (cache->dh > 128 || cache->dh % vec != 0)
+        return fail(NTSAMD_ERR_ARGUMENT, "head size %d is not served by the cache (a multiple of %d up to 128 is)", cache->dh, vec);
+    if (!cache->k || !cache->v || !batch->lengths || (!batch->pageTable && batch->tablePages > 0))
+        return fail(NTSAMD_ERR_ARGUMENT, "Empty input tensors!");
+    if (!aligned16(cache->k) || !aligned16(cache->v))
+        return fail(NTSAMD_ERR_ARGUMENT, "the cache must be 16-byte aligned");
+    const void * ints[3] = {batch->lengths, batch->starts, batch->pageTable};
+    for (int i = 0; i < 3; i++)
+        if ((reinterpret_cast<uintptr_t>(ints[i]) & 3) != 0)
+            return fail(NTSAMD_ERR_ARGUMENT, "misaligned lengths, starts or page table");
+    for (int i = 0; i < 6; i++)
+        if (cache->strides[i] < 0 || cache->strides[i] % vec != 0)
+            return fail(NTSAMD_ERR_ARGUMENT, "strides must be non-negative multiples of %d elements", vec);
+    const long long counts[3] = {cache->pages, cache->pageSize, cache->heads};
+    if (rows_overlap(cache->strides, counts, 3, cache->dh) || rows_overlap(cache->strides + 3, counts, 3, cache->dh))
+        return fail(NTSAMD_ERR_ARGUMENT, "rows of the cache overlap");
+    const long long positions = (long long)batch->tablePages * cache->pageSize;
+    if (batch->maxLength > positions)
+        return fail(NTSAMD_ERR_ARGUMENT, "sequences of %d positions, but %d pages of %d in a row of the page table",
+                    batch->maxLength, batch->tablePages, cache->pageSize);
+    const long long maxLength = batch->maxLength > 0 ? batch->maxLength : positions;
+    if (maxLength > 0x7fff0000LL)
+        return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
+    if (!batch->starts && (long long)batch->sequences * batch->maxNew > batch->tokens)
+        return fail(NTSAMD_ERR_ARGUMENT, "%d sequences of %d new tokens, but %d rows", batch->sequences, batch->maxNew, batch->tokens);
+    c.k = cache->k;
+    c.v = cache->v;
+    c.kP = cache->strides[0]; c.kR = cache->strides[1]; c.kH = cache->strides[2];
+    c.vP = cache->strides[3]; c.vR = cache->strides[4]; c.vH = cache->strides[5];
+    c.pages = cache->pages;
+    c.kvHeads = cache->heads;
+    c.dh = cache->dh;
+    c.pageSize = fast_div(cache->pageSize);
+    c.lengths = batch->lengths;
+    c.starts = batch->starts;
+    c.table = batch->pageTable;
+    c.sequences = batch->sequences;
+    c.tablePages = batch->tablePages;
+    c.tokens = batch->tokens;
+    c.maxNew = batch->maxNew < batch->tokens ? batch->maxNew : batch->tokens;
+    c.maxLength = (int)maxLength;
+    return NTSAMD_OK;
+}
+
+/* How the rows and keys of a cached attention are dealt out (see attention_cached.hip for the forms). */
+constexpr int CACHED_UNIT_HALF = 32, CACHED_UNIT_FLOAT = 16;
+
+int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool half, int prefix)
+{
+    const int unit = half ? CACHED_UNIT_HALF : CACHED_UNIT_FLOAT, qrMost = half ? 4 : 2;
+    const int kv = p.c.kvHeads, dh = p.c.dh, n = p.c.sequences;
+    const long long rows = (long long)p.c.maxNew * p.per;           /* of one sequence and key head, at most */
+    int cus = devID >= 0 && devID < MAX_DEVICES ? g_deviceCUs[devID].load(std::memory_order_relaxed) : 0;
+    if (cus <= 0)
+        cus = 256;
+    const long long slotRow = (long long)(dh + 2) * 4;              /* bytes of a partial row */
+    const bool mayHold = tuning().splitK.load(std::memory_order_relaxed) != 1;
+    const auto units = [unit](long long keys) { return (keys + unit - 1) / unit; };
+    const auto blocks_of = [](long long r) { return r <= 16 ? 1 : (r <= 32 ? 2 : 4); };
+    WorkHold work;
+    int rc = 0;
+    char text[160] = "";
+    p.seq0 = 0;
+    p.seqs = n;
+    p.first = 0;
+    p.prefix = 0;
+    p.acc = p.stat = NULL;
+    prefix = prefix < p.c.maxLength ? prefix : p.c.maxLength;
+
+    if (rows > 16 * qrMost) {
+        /* many rows to a sequence: tiles of rows, their keys in one piece where the tiles fill the part */
+        p.mode = CACHED_TILES;
+        p.rows = 16 * qrMost;
+        const long long perSeq = (rows + p.rows - 1) / p.rows;
+        long long tiles = (long long)p.c.tokens * p.per / p.rows + n;
+        if (!p.c.starts || n * perSeq < tiles)
+            tiles = n * perSeq;
+        long long pieces = 1;
+        if (mayHold && tiles * kv < 2 * cus) {
+            pieces = (2 * cus + tiles * kv - 1) / (tiles * kv);
+            const long long most = (units(p.c.maxLength) + 15) / 16, fit = (long long)SPLIT_WORK_BYTES / (tiles * kv * p.rows * slotRow);
+            pieces = pieces < most ? pieces : most;
+            pieces = pieces < fit ? pieces : fit;
+            if (pieces > 1) {
+                work.take_stream(devID, stream);
+                if (work.mem == NULL)
+                    pieces = 1;
+            }
+            else
+                pieces = 1;
+        }
+        if (tiles * kv * pieces > 0x7fffffffLL || (pieces > 1 && tiles * kv * p.rows > 0x7fffffffLL))
+            return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
+        p.tiles = (int)tiles;
+        p.groups = (int)pieces;
+        if (pieces > 1) {
+            p.acc = work.mem;
+            p.stat = p.acc + tiles * kv * pieces * p.rows * dh;
+        }
+        snprintf(g_plan, sizeof(g_plan), "attention_cached_kernel tiles=%lldx%d pieces=%lld%s", tiles, p.rows, pieces,
+                 pieces > 1 ? "+attention_join_kernel" : "");
+        if (g_planOnly)
+            return NTSAMD_OK;
+        rc = launch_attention_cached(p, half, qrMost, (int)(tiles * kv * pieces), stream);
+        if (rc == 0 && pieces > 1) {
+            JoinParams j;
+            memset(&j, 0, sizeof(j));
+            j.p = p;
+            rc = launch_attention_join(j, half, (int)(tiles * kv * p.rows), stream);
+        }
+    }
+    else {
+        const int qr = blocks_of(rows);
+        p.rows = (int)rows;
+        const long long room = (long long)SPLIT_WORK_BYTES / slotRow;       /* partial rows that fit */
+        const bool shared = prefix >= 4 * unit && n > 1 && mayHold && 256LL * kv <= room;
+        const long long own = p.c.maxLength - (shared ? prefix : 0);
+        bool flat = mayHold && units(own) > 8;
+        if (shared || flat) {
+            work.take_stream(devID, stream);
+            if (work.mem == NULL)
+                flat = false;
+        }
+        const bool withPrefix = shared && work.mem != NULL;
+        if (!withPrefix)
+            flat = mayHold && work.mem != NULL && units(p.c.maxLength) > 8;
+        /* with a prefix every row has a partial result of its own keys beside those of the prefix's pieces */
+        int step = n;
+        if (withPrefix) {
+            const long long most = room / 4 / (rows * kv);
+            step = most < n ? (most > 1 ? (int)most : 1) : n;
+        }
+        if (!withPrefix)
+            prefix = 0;
+        if ((long long)step * kv * rows > 0x7fffffffLL / 64)
+            return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
+        for (int seq0 = 0; seq0 < n && rc == 0; seq0 += step) {
+            CachedParams o = p;
+            o.seq0 = seq0;
+            o.seqs = n - seq0 < step ? n - seq0 : step;
+            const long long pairs = (long long)o.seqs * kv;
+            JoinParams j;
+            memset(&j, 0, sizeof(j));
+            long long used = 0;
+            if (withPrefix) {
+                CachedParams s = o;
+                const long long all = o.seqs * rows;
+                const int sqr = all <= 16 ? 1 : (all <= 32 || qrMost == 2 ? 2 : 4);
+                s.mode = CACHED_TILES;
+                s.prefix = prefix;
+                s.rows = 16 * sqr;
+                s.tiles = (int)((all + s.rows - 1) / s.rows);
+                const long long slots = (long long)s.tiles * kv;
+                long long pieces = (2 * cus + slots - 1) / slots;
+                const long long most = (units(prefix) + 3) / 4, fit = room / 2 / (slots * s.rows);
+                pieces = pieces < most ? pieces : most;
+                pieces = pieces < fit ? pieces : fit;
+                if (pieces < 1)
+                    pieces = 1;
+                s.groups = (int)pieces;
+                s.acc = work.mem;
+                s.stat = s.acc + slots * pieces * s.rows * dh;
+                used = slots * pieces * s.rows;
+                j.preAcc = s.acc;
+                j.preStat = s.stat;
+                j.prePieces = s.groups;
+                j.preRows = s.rows;
+                snprintf(text, sizeof(text), "attention_cached_kernel prefix tiles=%dx%d pieces=%lld+", s.tiles, s.rows, pieces);
+                if (!g_planOnly)
+                    rc = launch_attention_cached(s, half, sqr, (int)(slots * pieces), stream);
+            }
+            o.first = prefix;
+            long long blocks = pairs;
+            o.mode = CACHED_WHOLE;
+            if (flat) {
+                /* two workgroups to a CU, in rounds of a unit to a wave; their slots, and one for each pair behind a prefix */
+                const long long left = room - used - (withPrefix ? pairs * rows : 0);
+                long long groups = 2 * cus, need = (pairs * units(own) + 3) / 4;
+                groups = groups < need ? groups : need;
+                groups = groups < left / (2 * rows) ? groups : left / (2 * rows);
+                if (groups >= 1) {
+                    o.mode = CACHED_FLAT;
+                    o.groups = (int)groups;
+                    blocks = groups;
+                }
+            }
+            if (withPrefix || o.mode == CACHED_FLAT) {
+                const long long slots = (o.mode == CACHED_FLAT ? 2 * blocks : 0) + (withPrefix ? pairs : 0);
+                o.acc = work.mem + used * (dh + 2);
+                o.stat = o.acc + slots * rows * dh;
+            }
+            snprintf(g_plan, sizeof(g_plan), "%sattention_cached_kernel rows=%d %s=%lld%s", text, 16 * qr,
+                     o.mode == CACHED_FLAT ? "flat" : "whole", blocks, o.acc ? "+attention_join_kernel" : "");
+            if (g_planOnly)
+                return NTSAMD_OK;
+            if (rc == 0)
+                rc = launch_attention_cached(o, half, qr, (int)blocks, stream);
+            if (rc == 0 && o.acc) {
+                j.p = o;
+                rc = launch_attention_join(j, half, (int)(pairs * rows), stream);
+            }
+        }
+    }
+    if (rc != 0)
+        return fail(NTSAMD_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString((hipError_t)rc));
+    return NTSAMD_OK;
+}
+
+int attention_over_cache(int devID, void * stream, const ntsamd_cache * cache, const ntsamd_cache_batch * batch,
+                         const void * q, void * out, int heads, const long long * strides, float scale, int causal, int prefix)
+{
+    CachedParams p;
+    memset(&p, 0, sizeof(p));
+    bool empty;
+    int st = check_cache(cache, batch, p.c, empty);
+    if (st != NTSAMD_OK)
+        return st;
+    if (heads < 0)
+        return fail(NTSAMD_ERR_ARGUMENT, "negative tensor size");
+    if (prefix < 0)
+        return fail(NTSAMD_ERR_ARGUMENT, "negative length of the prefix");
+    if (empty || heads == 0)
+        return NTSAMD_OK;
+    if (heads % p.c.kvHeads != 0)
+        return fail(NTSAMD_ERR_ARGUMENT, "%d heads cannot share %d key heads evenly", heads, p.c.kvHeads);
+    if (!q || !out || !strides)
+        return fail(NTSAMD_ERR_ARGUMENT, "Empty input tensors!");
+    const bool half = cache->dataType == NTSAMD_X_FLOAT16;
+    const int vec = half ? 8 : 4;
+    if (!aligned16(q) || !aligned16(out))
+        return fail(NTSAMD_ERR_ARGUMENT, "q and out must be 16-byte aligned");
+    for (int i = 0; i < 4; i++)
+        if (strides[i] < 0 || strides[i] % vec != 0)
+            return fail(NTSAMD_ERR_ARGUMENT, "strides must be non-negative multiples of %d elements", vec);
+    const long long counts[2] = {p.c.tokens, heads};
+    if (rows_overlap(strides + 2, counts, 2, p.c.dh))
+        return fail(NTSAMD_ERR_ARGUMENT, "rows of the result overlap");
+    p.per = heads / p.c.kvHeads;
+    if ((long long)p.c.tokens * p.per > 0x7fff0000LL)
+        return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
+    const bool planOnly = g_planOnly;
+    if (!planOnly) {
+        st = check_device(devID);
+        if (st != NTSAMD_OK)
+            return st;
+    }
+    DeviceScope scope(devID, planOnly);
+    if (scope.status != NTSAMD_OK)
+        return scope.status;
+    p.q = q;
+    p.out = out;
+    p.qT = strides[0]; p.qH = strides[1]; p.oT = strides[2]; p.oH = strides[3];
+    p.perDiv = fast_div(p.per);
+    p.scale = scale;
+    p.causal = causal != 0;
+    return run_attention_cached(devID, static_cast<hipStream_t>(stream), p, half, prefix);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1427,6 +1732,88 @@ int ntsamd_attention_train(int devID, void * stream,
     if (rc != 0)
         return fail(NTSAMD_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString((hipError_t)rc));
     return NTSAMD_OK;
+}
+
+int ntsamd_cache_append(int devID, void * stream, const ntsamd_cache * cache, const ntsamd_cache_batch * batch,
+                        const void * k, const void * v, const void * q, void * qOut, int heads,
+                        const long long * strides,
+                        const float * rotation, int positions, int rotated, int pairing)
+{
+    AppendParams p;
+    memset(&p, 0, sizeof(p));
+    bool empty;
+    int st = check_cache(cache, batch, p.c, empty);
+    if (st != NTSAMD_OK)
+        return st;
+    if ((q && heads < 0) || (rotation && positions < 0))
+        return fail(NTSAMD_ERR_ARGUMENT, "negative tensor size");
+    if (empty)
+        return NTSAMD_OK;
+    if (!k || !v || !strides || (q != NULL) != (qOut != NULL))
+        return fail(NTSAMD_ERR_ARGUMENT, "Empty input tensors!");
+    if (rotation && (rotated < 0 || rotated % 2 != 0 || rotated > p.c.dh))
+        return fail(NTSAMD_ERR_ARGUMENT, "%d rotated columns (an even number up to the head size %d)", rotated, p.c.dh);
+    if (rotation && pairing != NTSAMD_ROTATE_HALVES && pairing != NTSAMD_ROTATE_PAIRS)
+        return fail(NTSAMD_ERR_ARGUMENT, "unknown pairing %d of rotated columns", pairing);
+    const bool half = cache->dataType == NTSAMD_X_FLOAT16;
+    const uintptr_t size = half ? 2 : 4;
+    if (reinterpret_cast<uintptr_t>(k) % size != 0 || reinterpret_cast<uintptr_t>(v) % size != 0 ||
+        reinterpret_cast<uintptr_t>(q) % size != 0 || reinterpret_cast<uintptr_t>(qOut) % size != 0 ||
+        reinterpret_cast<uintptr_t>(rotation) % 4 != 0)
+        return fail(NTSAMD_ERR_ARGUMENT, "misaligned tensor data");
+    for (int i = 0; i < (q ? 8 : 4); i++)
+        if (strides[i] < 0)
+            return fail(NTSAMD_ERR_ARGUMENT, "negative stride");
+    if (q) {
+        const long long counts[2] = {p.c.tokens, heads};
+        if (rows_overlap(strides + 6, counts, 2, p.c.dh))
+            return fail(NTSAMD_ERR_ARGUMENT, "rows of the result overlap");
+        if (q == qOut && (strides[4] != strides[6] || strides[5] != strides[7]))
+            return fail(NTSAMD_ERR_ARGUMENT, "queries turned in place keep their strides");
+    }
+    const bool planOnly = g_planOnly;
+    if (!planOnly) {
+        st = check_device(devID);
+        if (st != NTSAMD_OK)
+            return st;
+    }
+    DeviceScope scope(devID, planOnly);
+    if (scope.status != NTSAMD_OK)
+        return scope.status;
+    p.nk = k;
+    p.nv = v;
+    p.q = heads > 0 ? q : NULL;
+    p.qOut = qOut;
+    p.heads = heads;
+    p.kT = strides[0]; p.kH = strides[1]; p.vT = strides[2]; p.vH = strides[3];
+    if (q) {
+        p.qT = strides[4]; p.qH = strides[5]; p.oT = strides[6]; p.oH = strides[7];
+    }
+    p.rotation = rotation;
+    p.positions = positions;
+    p.rotated = rotation ? rotated : 0;
+    p.pairing = pairing;
+    snprintf(g_plan, sizeof(g_plan), "cache_append_kernel");
+    if (planOnly)
+        return NTSAMD_OK;
+    int rc = launch_cache_append(p, half, static_cast<hipStream_t>(stream));
+    if (rc != 0)
+        return fail(NTSAMD_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString((hipError_t)rc));
+    return NTSAMD_OK;
+}
+
+int ntsamd_attention_cached(int devID, void * stream, const ntsamd_cache * cache, const ntsamd_cache_batch * batch,
+                            const void * q, void * out, int heads, const long long * strides,
+                            float scale, int causal)
+{
+    return attention_over_cache(devID, stream, cache, batch, q, out, heads, strides, scale, causal, 0);
+}
+
+int ntsamd_attention_prefix(int devID, void * stream, const ntsamd_cache * cache, const ntsamd_cache_batch * batch,
+                            const void * q, void * out, int heads, const long long * strides,
+                            float scale, int causal, int prefix)
+{
+    return attention_over_cache(devID, stream, cache, batch, q, out, heads, strides, scale, causal, prefix);
 }
 
 int ntsamd_matrix_mul(int devID, void * stream,
