@@ -7,9 +7,7 @@
 
 namespace ntsamd {
 
-struct CachedShared {
-    float acc[4][16][132];
-    float stat[4][16][2];
+struct CachedScan {
     long long sums[4];
     long long before;
     int found;
@@ -29,7 +27,7 @@ struct SequenceScan {
 };
 
 template <typename W>
-__device__ __forceinline__ SequenceScan scan_sequences(int count, CachedShared & sh, W weight)
+__device__ __forceinline__ SequenceScan scan_sequences(int count, CachedScan & sh, W weight)
 {
     SequenceScan r;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -62,7 +60,7 @@ __device__ __forceinline__ SequenceScan scan_sequences(int count, CachedShared &
 
 /* the sequence of a launch in which place `at` of the sum falls, and the sum before it; -1 past the end */
 template <typename W>
-__device__ __forceinline__ int find_sequence(const SequenceScan & r, long long at, long long & before, CachedShared & sh, W weight)
+__device__ __forceinline__ int find_sequence(const SequenceScan & r, long long at, long long & before, CachedScan & sh, W weight)
 {
     if (at >= r.total)
         return -1;
@@ -92,13 +90,22 @@ struct FlatPlan {
 
 /* a workgroup's four waves take a unit each at a time: no more workgroups than whole rounds */
 template <int UK>
-__device__ __forceinline__ FlatPlan flat_plan(const CachedParams & p, CachedShared & sh)
+__device__ __forceinline__ FlatPlan flat_plan(const CachedParams & p, CachedScan & sh)
 {
     FlatPlan f;
     f.scan = scan_sequences(p.seqs, sh, [&](int i) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)) * p.c.kvHeads; });
     f.groups = (int)min((long long)p.groups, (f.scan.total + 3) / 4);
     return f;
 }
+
+/* a range of the keys of one tile of rows */
+struct Segment {
+    CacheSequence s;
+    int seq, head;                      /* table row, key head */
+    int row0, rows;                     /* first row of the tile, rows the sequence has */
+    int u0, u1;                         /* units, from p.first on */
+    int slot;                           /* where the partial result goes, -1: the result goes to out */
+};
 
 /* tokens of the sequences of a launch, which begin at row `start` */
 __device__ __forceinline__ int prefix_tokens(const CachedParams & p, int start)
@@ -109,7 +116,130 @@ __device__ __forceinline__ int prefix_tokens(const CachedParams & p, int start)
     return min(max(min(p.c.starts[p.seq0 + p.seqs], p.c.tokens) - start, 0), most);
 }
 
+/* CACHED_TILES: the segment of workgroup `id`, tiles of TR rows, units of UK keys; false: it has none */
+template <int TR, int UK>
+__device__ __forceinline__ bool tile_segment(const CachedParams & p, CachedScan & sh, int id, Segment & sg)
+{
+    /* the last tiles of a sequence see the most keys: first */
+    const int perTile = p.c.kvHeads * p.groups;
+    int tile = p.tiles - 1 - id / perTile;
+    const int rest = id % perTile, piece = rest / p.c.kvHeads;
+    sg.head = rest - piece * p.c.kvHeads;
+    sg.slot = p.acc ? (tile * p.c.kvHeads + sg.head) * p.groups + piece : -1;
+    if (p.prefix > 0) {
+        sg.s.start = cache_sequence(p.c, p.seq0).start;
+        sg.s.fresh = prefix_tokens(p, sg.s.start);
+        sg.s.length = p.prefix;
+        sg.seq = 0;
+    }
+    else {
+        const auto tiles = [&](int n) { return (long long)((cache_sequence(p.c, p.seq0 + n).fresh * p.per + TR - 1) / TR); };
+        const SequenceScan scan = scan_sequences(p.seqs, sh, tiles);
+        long long before;
+        const int i = find_sequence(scan, tile, before, sh, tiles);
+        if (i < 0)
+            return false;
+        tile -= (int)before;
+        sg.seq = p.seq0 + i;
+        sg.s = cache_sequence(p.c, sg.seq);
+    }
+    sg.rows = sg.s.fresh * p.per;
+    sg.row0 = tile * TR;
+    if (sg.row0 >= sg.rows)
+        return false;
+    int keys = sg.s.length;
+    if (p.causal && p.prefix == 0)
+        keys -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
+    const int units = (max(keys - p.first, 0) + UK - 1) / UK;
+    sg.u0 = (int)((long long)units * piece / p.groups);
+    sg.u1 = (int)((long long)units * (piece + 1) / p.groups);
+    return true;
+}
+
+/* The sequences of this lane's rows (row0 + 16 q) in a launch over the shared prefix, whose rows are the tokens of all
+   sequences: the last one that starts at or before the row's token, searched for in LDS (`from`, N of them at a time). */
+template <int QR, int N>
+__device__ __forceinline__ void row_sequences(const CachedParams & p, const Segment & sg, int row0, int * from, int (&seq)[QR])
+{
+    int tok[QR], count[QR];
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const int row = row0 + 16 * q;
+        tok[q] = sg.s.start + (row < sg.rows ? divided(row, p.perDiv) : 0);
+        count[q] = 0;
+    }
+    for (int i0 = 0; i0 < p.seqs; i0 += N) {
+        const int n = min(N, p.seqs - i0);
+        for (int i = threadIdx.x; i < n; i += 256)
+            from[i] = p.c.starts[p.seq0 + i0 + i];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < QR; q++) {
+            int lo = 0, hi = n;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (from[mid] <= tok[q])
+                    lo = mid + 1;
+                else
+                    hi = mid;
+            }
+            count[q] += lo;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < QR; q++)
+        seq[q] = p.seq0 + max(count[q] - 1, 0);
+}
+
+/* How many positions this lane's rows (row0 + 16 q) see, the least and the most of the 16 lanes' rows. Rows that a
+   tile does not have see everything: they are computed with, never stored. */
+template <int QR, int N>
+__device__ __forceinline__ void rows_seen(const CachedParams & p, const Segment & sg, int row0, int * from, int (&seen)[QR],
+                                          int & least, int & most)
+{
+    if (p.prefix > 0 && p.c.starts)
+        row_sequences<QR, N>(p, sg, row0, from, seen);
+    least = 0x7fffffff;
+    most = 0;
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const int row = row0 + 16 * q, t = divided(row, p.perDiv);
+        if (row >= sg.rows) {
+            seen[q] = 0x7fffffff;
+            continue;
+        }
+        if (p.prefix > 0) {
+            const CacheSequence s = cache_sequence(p.c, p.c.starts ? seen[q] : p.seq0 + t / p.c.maxNew);
+            seen[q] = min(p.causal ? s.length - s.fresh + (sg.s.start + t - s.start) + 1 : s.length, p.prefix);
+        }
+        else
+            seen[q] = p.causal ? sg.s.length - sg.s.fresh + t + 1 : sg.s.length;
+        least = min(least, seen[q]);
+        most = max(most, seen[q]);
+    }
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) {
+        least = min(least, __shfl_xor(least, d));
+        most = max(most, __shfl_xor(most, d));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+}
+
+/* where positions that do not exist and columns past dh are read from */
+static __device__ const float zero_row[4] = {0.f, 0.f, 0.f, 0.f};
+
+__device__ __forceinline__ long long lane_of(long long x, int source)
+{
+    const int lo = __shfl((int)x, source), hi = __shfl((int)(x >> 32), source);
+    return ((long long)hi << 32) | (unsigned)lo;
+}
+
 int launch_attention_cached(const CachedParams & p, bool half, int qr, int blocks, hipStream_t stream);
+/* CACHED_TILES of half tensors, tiles of 64 qr rows (qr 1 or 2) */
+int launch_attention_cached_tiles(const CachedParams & p, int qr, int blocks, hipStream_t stream);
+constexpr int CACHED_TILE_KEYS = 64;
 
 /* the partial results of a launch (p.acc, p.stat), and of the launch over the shared prefix before it, to p.out */
 struct JoinParams {

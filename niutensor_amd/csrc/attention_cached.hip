@@ -32,8 +32,6 @@ namespace ntsamd {
 
 namespace {
 
-__device__ const float zero_row[4] = {0.f, 0.f, 0.f, 0.f};
-
 template <typename T, int DHM> struct Unit;
 template <int DHM> struct Unit<half_t, DHM> {
     static constexpr int UK = 32, NJ = 2;               /* keys, blocks of 16 of them */
@@ -58,11 +56,11 @@ template <typename T, int DHM> struct UnitData {
     unsigned there;                                     /* which of its keys exist */
 };
 
-__device__ __forceinline__ long long lane_of(long long x, int source)
-{
-    const int lo = __shfl((int)x, source), hi = __shfl((int)(x >> 32), source);
-    return ((long long)hi << 32) | (unsigned)lo;
-}
+struct CachedShared {
+    float acc[4][16][132];
+    float stat[4][16][2];
+    CachedScan scan;
+};
 
 /* ND columns from `col` on, those below dh, times f */
 template <typename T, int ND>
@@ -81,55 +79,6 @@ __device__ __forceinline__ void store_columns(T * row, int col, int dh, const fl
         }
 }
 
-/* a range of the keys of one tile of rows */
-struct Segment {
-    CacheSequence s;
-    int seq, head;                      /* table row, key head */
-    int row0, rows;                     /* first row of the tile, rows the sequence has */
-    int u0, u1;                         /* units, from p.first on */
-    int slot;                           /* where the partial result goes, -1: the result goes to out */
-};
-
-/* The sequences of this lane's rows in a launch over the shared prefix, whose rows are the tokens of all sequences: the
-   last one that starts at or before the row's token, searched for in LDS. */
-template <int QR>
-__device__ __forceinline__ void row_sequences(const CachedParams & p, const Segment & sg, CachedShared & sh, int (&seq)[QR])
-{
-    constexpr int N = 4096;
-    static_assert(N * sizeof(int) <= sizeof(sh.acc), "");
-    int * from = reinterpret_cast<int *>(&sh.acc[0][0][0]);
-    const int m = threadIdx.x & 15;
-    int tok[QR], count[QR];
-#pragma unroll
-    for (int q = 0; q < QR; q++) {
-        const int row = sg.row0 + 16 * q + m;
-        tok[q] = sg.s.start + (row < sg.rows ? divided(row, p.perDiv) : 0);
-        count[q] = 0;
-    }
-    for (int i0 = 0; i0 < p.seqs; i0 += N) {
-        const int n = min(N, p.seqs - i0);
-        for (int i = threadIdx.x; i < n; i += 256)
-            from[i] = p.c.starts[p.seq0 + i0 + i];
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < QR; q++) {
-            int lo = 0, hi = n;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (from[mid] <= tok[q])
-                    lo = mid + 1;
-                else
-                    hi = mid;
-            }
-            count[q] += lo;
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int q = 0; q < QR; q++)
-        seq[q] = p.seq0 + max(count[q] - 1, 0);
-}
-
 template <typename T, int DHM, int QR>
 __device__ __forceinline__ void attend(const CachedParams & p, const Segment & sg, CachedShared & sh)
 {
@@ -143,25 +92,15 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     const int dh = c.dh;
 
     /* ---- this lane's query rows: positions each sees, fragments ---- */
-    int seen[QR] = {};
+    int seen[QR], seenMin, seenMax;
+    rows_seen<QR, 4096>(p, sg, sg.row0 + m, reinterpret_cast<int *>(&sh.acc[0][0][0]), seen, seenMin, seenMax);
     typename U::KPiece qf[QR][U::NT];
-    if (p.prefix > 0 && c.starts)
-        row_sequences<QR>(p, sg, sh, seen);             /* for now: the sequence of each row */
 #pragma unroll
     for (int q = 0; q < QR; q++) {
         const int row = sg.row0 + 16 * q + m;
         const bool there = row < sg.rows;
         const int t = there ? divided(row, p.perDiv) : 0;
         const int h = sg.head * p.per + (there ? row - t * p.per : 0);
-        if (!there)
-            seen[q] = 0x7fffffff;                       /* padding: computed with, never stored */
-        else if (p.prefix > 0) {
-            const int seq = c.starts ? seen[q] : p.seq0 + t / c.maxNew;
-            const CacheSequence s = cache_sequence(c, seq);
-            seen[q] = min(p.causal ? s.length - s.fresh + (sg.s.start + t - s.start) + 1 : s.length, p.prefix);
-        }
-        else
-            seen[q] = p.causal ? sg.s.length - sg.s.fresh + t + 1 : sg.s.length;
         const T * qr = static_cast<const T *>(p.q) + (long long)(sg.s.start + t) * p.qT + h * p.qH;
 #pragma unroll
         for (int t4 = 0; t4 < U::NT; t4++) {
@@ -171,19 +110,6 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
             qf[q][t4] = there && col < dh ? *reinterpret_cast<const typename U::KPiece *>(qr + col) : z;
         }
     }
-    int seenMin = seen[0], seenMax = 0;
-#pragma unroll
-    for (int q = 0; q < QR; q++) {
-        seenMin = min(seenMin, seen[q]);
-        seenMax = max(seenMax, seen[q] == 0x7fffffff ? 0 : seen[q]);
-    }
-#pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) {
-        seenMin = min(seenMin, __shfl_xor(seenMin, d));
-        seenMax = max(seenMax, __shfl_xor(seenMax, d));
-    }
-    seenMin = __builtin_amdgcn_readfirstlane(seenMin);
-    seenMax = __builtin_amdgcn_readfirstlane(seenMax);
 
     /* ---- loading a unit ---- */
     const int * table = c.table + (long long)sg.seq * c.tablePages;
@@ -398,7 +324,7 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
 }
 
 template <typename T, int DHM, int QR>
-__global__ void __launch_bounds__(256, QR == 1 ? 2 : 1)
+__global__ void __launch_bounds__(256, QR == 2 && DHM == 128 ? 1 : 2)
 attention_cached_kernel(const CachedParams p)
 {
     constexpr int UK = Unit<T, DHM>::UK, TR = 16 * QR;
@@ -419,12 +345,12 @@ attention_cached_kernel(const CachedParams p)
             attend<T, DHM, QR>(p, sg, sh);
     }
     else if (p.mode == CACHED_FLAT) {
-        const FlatPlan f = flat_plan<UK>(p, sh);
+        const FlatPlan f = flat_plan<UK>(p, sh.scan);
         if (id >= f.groups)
             return;
         const long long begin = f.start(id), end = f.start(id + 1);
         long long before;
-        int i = find_sequence(f.scan, begin, before, sh,
+        int i = find_sequence(f.scan, begin, before, sh.scan,
                               [&](int n) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + n)) * p.c.kvHeads; });
         for (long long at = begin; at < end;) {
             sg.seq = p.seq0 + i;
@@ -449,40 +375,8 @@ attention_cached_kernel(const CachedParams p)
         }
     }
     else {
-        /* the last tiles of a sequence see the most keys: first */
-        const int perTile = p.c.kvHeads * p.groups;
-        int tile = p.tiles - 1 - id / perTile;
-        const int rest = id % perTile, piece = rest / p.c.kvHeads;
-        sg.head = rest - piece * p.c.kvHeads;
-        const int slot = (tile * p.c.kvHeads + sg.head) * p.groups + piece;
-        if (p.prefix > 0) {
-            sg.s.start = cache_sequence(p.c, p.seq0).start;
-            sg.s.fresh = prefix_tokens(p, sg.s.start);
-            sg.s.length = p.prefix;
-            sg.seq = 0;
-        }
-        else {
-            const auto tiles = [&](int n) { return (long long)((cache_sequence(p.c, p.seq0 + n).fresh * p.per + TR - 1) / TR); };
-            const SequenceScan scan = scan_sequences(p.seqs, sh, tiles);
-            long long before;
-            const int i = find_sequence(scan, tile, before, sh, tiles);
-            if (i < 0)
-                return;
-            tile -= (int)before;
-            sg.seq = p.seq0 + i;
-            sg.s = cache_sequence(p.c, sg.seq);
-        }
-        sg.rows = sg.s.fresh * p.per;
-        sg.row0 = tile * TR;
-        if (sg.row0 >= sg.rows)
+        if (!tile_segment<TR, UK>(p, sh.scan, id, sg))
             return;
-        int keys = sg.s.length;
-        if (p.causal && p.prefix == 0)
-            keys -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
-        const int units = (max(keys - p.first, 0) + UK - 1) / UK;
-        sg.u0 = (int)((long long)units * piece / p.groups);
-        sg.u1 = (int)((long long)units * (piece + 1) / p.groups);
-        sg.slot = p.acc ? slot : -1;
         attend<T, DHM, QR>(p, sg, sh);
     }
 }
@@ -493,10 +387,8 @@ int launch_dhm(const CachedParams & p, int qr, int blocks, hipStream_t stream)
     const dim3 grid((unsigned)blocks), block(256);
     if (qr == 1)
         hipLaunchKernelGGL((attention_cached_kernel<T, DHM, 1>), grid, block, 0, stream, p);
-    else if (qr == 2)
-        hipLaunchKernelGGL((attention_cached_kernel<T, DHM, 2>), grid, block, 0, stream, p);
     else
-        hipLaunchKernelGGL((attention_cached_kernel<T, DHM, 4>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((attention_cached_kernel<T, DHM, 2>), grid, block, 0, stream, p);
     return (int)hipGetLastError();
 }
 

@@ -1,0 +1,279 @@
+/*
+ * Attention over a cache on pages for many query rows in half: pieces of text against what is in the cache, and the
+ * queries of a whole batch against a prefix they share (ntsamd_attention_cached, ntsamd_attention_prefix; the few rows of a
+ * decoding step and float go to attention_cached.hip).
+ *
+ * Bound by the matrix instructions and what feeds them, so keys and values go through LDS once for all rows of a
+ * workgroup, on the plan of attention_f16.hip: 64 QR rows (tokens x the query heads that share a key head) of a tile, 16 QR
+ * per wave; blocks of 64 keys; both products transposed, so that probabilities pass from accumulator to operand inside
+ * a lane; values read back by transposing LDS reads. What is different is where the keys stand: lane l of every wave looks
+ * up the page of key l of a block, one block ahead, and hands its address to the lanes that fetch the row. Rows of a
+ * tile see different numbers of keys; only the blocks in which some row's last key falls, or which have an absent page, take the
+ * comparisons. Fetches of keys that a tile does not have read a row of zeros.
+ */
+#include "gemm_common.h"
+#include "gemm_f16.h"       /* half_t, lds_read_tr16 */
+#include "attention.h"
+#include "attention_cached.h"
+
+namespace ntsamd {
+
+namespace {
+
+template <int DHM, int QR>
+__global__ void __launch_bounds__(256, QR == 2 && DHM <= 64 ? 3 : 2)
+attention_cached_tiles_kernel(const CachedParams p)
+{
+    constexpr int KB = CACHED_TILE_KEYS, TR = 64 * QR;
+    constexpr int PITCH = DHM * 2 + 16;      /* bytes per LDS row: 16 mod 128, so 16-byte reads of consecutive rows
+                                                walk through the banks */
+    constexpr int NT = DHM / 32, ND = DHM / 16, NJ = KB / 16;
+    constexpr int TPR = DHM / 8;             /* threads per row when staging */
+    constexpr int RSTEP = 256 / TPR, LOADS = KB / RSTEP;
+    constexpr float LOG2E = 1.4426950408889634f;
+
+    __shared__ __attribute__((aligned(16))) char Ks[KB * PITCH];
+    __shared__ __attribute__((aligned(16))) char Vs[KB * PITCH];
+    __shared__ CachedScan scan;
+
+    const CacheParams & c = p.c;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    const int dh = c.dh;
+
+    Segment sg;
+    if (!tile_segment<TR, KB>(p, scan, (int)blockIdx.x, sg))
+        return;
+    const int row0 = sg.row0 + wave * (16 * QR) + m;
+    int seen[QR], seenMin, seenMax;
+    rows_seen<QR, KB * PITCH / 4>(p, sg, row0, reinterpret_cast<int *>(Ks), seen, seenMin, seenMax);
+
+    /* ---- where the keys of a block stand: lane l looks after key l ---- */
+    const int * table = c.table + (long long)sg.seq * c.tablePages;
+    const half_t * kBase = static_cast<const half_t *>(c.k) + sg.head * c.kH;
+    const half_t * vBase = static_cast<const half_t *>(c.v) + sg.head * c.vH;
+    const half_t * zero = reinterpret_cast<const half_t *>(zero_row);
+    int keyEnd = sg.s.length;                /* the keys that any row of the tile sees */
+    if (p.causal && p.prefix == 0)
+        keyEnd -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
+    auto page_of = [&](int u) {
+        const int key = p.first + u * KB + lane;
+        return u < sg.u1 && key < keyEnd ? table[divided(key, c.pageSize)] : -1;
+    };
+    const int sr0 = tid / TPR, sc = (tid % TPR) * 8;
+    const int sLds = sr0 * PITCH + sc * 2;
+    f16x8 kreg[LOADS], vreg[LOADS];
+    unsigned long long there = 0;            /* which keys of the block being fetched exist */
+    long long vOff;
+    auto load_k = [&](int u, int page) {
+        const int key = p.first + u * KB + lane;
+        const bool valid = page >= 0 && page < c.pages;
+        const int r = key - divided(key, c.pageSize) * (int)c.pageSize.d;
+        const long long kOff = valid ? page * c.kP + r * c.kR : -1;
+        vOff = valid ? page * c.vP + r * c.vR : -1;
+        there = __ballot(valid);
+#pragma unroll
+        for (int s = 0; s < LOADS; s++) {
+            const long long off = lane_of(kOff, sr0 + s * RSTEP);
+            kreg[s] = *reinterpret_cast<const f16x8 *>(off >= 0 && sc < dh ? kBase + off + sc : zero);
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int s = 0; s < LOADS; s++) {
+            const long long off = lane_of(vOff, sr0 + s * RSTEP);
+            vreg[s] = *reinterpret_cast<const f16x8 *>(off >= 0 && sc < dh ? vBase + off + sc : zero);
+        }
+    };
+    int page = page_of(sg.u0);
+    load_k(sg.u0, page);
+    page = page_of(sg.u0 + 1);
+
+    /* ---- Q fragments ---- */
+    f16x8 qf[QR][NT];
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const int row = row0 + 16 * q;
+        const bool has = row < sg.rows;
+        const int t = has ? divided(row, p.perDiv) : 0;
+        const int h = sg.head * p.per + (has ? row - t * p.per : 0);
+        const half_t * qr = static_cast<const half_t *>(p.q) + (long long)(sg.s.start + t) * p.qT + h * p.qH;
+#pragma unroll
+        for (int t4 = 0; t4 < NT; t4++) {
+            const int col = 32 * t4 + 8 * g;
+            const f16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+            qf[q][t4] = has && col < dh ? *reinterpret_cast<const f16x8 *>(qr + col) : z;
+        }
+    }
+
+    f32x4 accO[QR][ND];
+    float rowMax[QR], rowSum[QR];
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            accO[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        rowMax[q] = -INFINITY;
+        rowSum[q] = 0.f;
+    }
+    const float scale2 = p.scale * LOG2E;
+    /* where this lane points for the transposing reads: row 4 g + (m / 4) of a 16-key block, columns 4 (m % 4) .. + 3 */
+    const int trOff = (4 * g + (m >> 2)) * PITCH + (m & 3) * 8;
+
+    for (int u = sg.u0; u < sg.u1; u++) {
+        const bool more = u + 1 < sg.u1;
+        const int key0 = p.first + u * KB;
+        const unsigned long long exist = there;
+#pragma unroll
+        for (int s = 0; s < LOADS; s++)
+            *reinterpret_cast<f16x8 *>(&Ks[sLds + s * RSTEP * PITCH]) = kreg[s];
+        load_v();                            /* of this block: they are due after the first product */
+        __syncthreads();
+        if (more)
+            load_k(u + 1, page);
+        page = page_of(u + 2);
+
+        /* ---- S^T = K Q^T ---- */
+        f32x4 accS[QR][NJ];
+#pragma unroll
+        for (int q = 0; q < QR; q++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+                accS[q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const f16x8 kf = *reinterpret_cast<const f16x8 *>(&Ks[(16 * j + m) * PITCH + 64 * t + 16 * g]);
+#pragma unroll
+                for (int q = 0; q < QR; q++)
+                    accS[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[q][t], accS[q][j], 0, 0, 0);
+            }
+
+        /* ---- running softmax of the lane's rows ---- */
+        f16x4 pf[QR][NJ];
+        const bool cut = exist != ~0ull || key0 + KB > seenMin;
+#pragma unroll
+        for (int q = 0; q < QR; q++) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+                accS[q][j] *= scale2;
+            if (cut) {
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int at = 16 * j + 4 * g + r;
+                        if (!((exist >> at) & 1) || key0 + at >= seen[q])
+                            accS[q][j][r] = -INFINITY;
+                    }
+            }
+            float mx = accS[q][0][0];
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    mx = fmaxf(mx, accS[q][j][r]);
+            const float newMax = fmaxf(rowMax[q], lane_groups_max(mx));
+            const float shift = newMax == -INFINITY ? 0.f : newMax;
+            const float corr = __builtin_amdgcn_exp2f(rowMax[q] - shift);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float e = __builtin_amdgcn_exp2f(accS[q][j][r] - shift);
+                    sum += e;
+                    pf[q][j][r] = (half_t)e;
+                }
+            rowSum[q] = rowSum[q] * corr + sum;          /* this lane's keys only: the four lanes of a row meet at the end */
+            rowMax[q] = newMax;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                accO[q][d] *= corr;
+        }
+
+#pragma unroll
+        for (int s = 0; s < LOADS; s++)
+            *reinterpret_cast<f16x8 *>(&Vs[sLds + s * RSTEP * PITCH]) = vreg[s];
+        __syncthreads();
+
+        /* ---- O^T += V^T P^T, 32 keys per MFMA: its k index 8 g + e stands for key 4 g + e of the first 16-key block of a
+           pair for e < 4 and for key 4 g + e - 4 of the second for e >= 4 ---- */
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2)
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const f16x4 lo = lds_read_tr16(reinterpret_cast<const half_t *>(&Vs[16 * j * PITCH + trOff + 32 * d]));
+                const f16x4 hi = lds_read_tr16(reinterpret_cast<const half_t *>(&Vs[16 * (j + 1) * PITCH + trOff + 32 * d]));
+                const f16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int q = 0; q < QR; q++) {
+                    const f16x8 pp = __builtin_shufflevector(pf[q][j], pf[q][j + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    accO[q][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp, accO[q][d], 0, 0, 0);
+                }
+            }
+    }
+
+    /* ---- register r of block d is column 16 d + 4 g + r of the lane's row ---- */
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const float total = lane_groups_sum(rowSum[q]);
+        const int row = row0 + 16 * q;
+        if (row >= sg.rows)
+            continue;
+        if (sg.slot < 0) {
+            const int t = divided(row, p.perDiv);
+            half_t * out = static_cast<half_t *>(p.out) + (long long)(sg.s.start + t) * p.oT + (sg.head * p.per + row - t * p.per) * p.oH;
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const int col = 16 * d + 4 * g;
+                if (col < dh) {
+                    f16x4 o;
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        o[r] = (half_t)(accO[q][d][r] * inv);
+                    *reinterpret_cast<f16x4 *>(out + col) = o;
+                }
+            }
+        }
+        else {
+            const long long at = (long long)sg.slot * TR + (row - sg.row0);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const int col = 16 * d + 4 * g;
+                if (col < dh)
+                    *reinterpret_cast<f32x4 *>(p.acc + at * dh + col) = accO[q][d];
+            }
+            if (g == 0) {
+                p.stat[2 * at] = rowMax[q];
+                p.stat[2 * at + 1] = total;
+            }
+        }
+    }
+}
+
+template <int DHM>
+int launch_dhm(const CachedParams & p, int qr, int blocks, hipStream_t stream)
+{
+    if (qr == 1)
+        hipLaunchKernelGGL((attention_cached_tiles_kernel<DHM, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((attention_cached_tiles_kernel<DHM, 2>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int launch_attention_cached_tiles(const CachedParams & p, int qr, int blocks, hipStream_t stream)
+{
+    if (p.c.dh <= 32)
+        return launch_dhm<32>(p, qr, blocks, stream);
+    if (p.c.dh <= 64)
+        return launch_dhm<64>(p, qr, blocks, stream);
+    return launch_dhm<128>(p, qr, blocks, stream);
+}
+
+}  // namespace ntsamd

@@ -18,7 +18,8 @@ template <typename T, int UK>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(const JoinParams j)
 {
-    __shared__ CachedShared sh;
+    __shared__ CachedScan sh;
+    __shared__ float partAcc[8][128], partStat[8][2];
     const CachedParams & p = j.p;
     const int id = (int)blockIdx.x, kv = p.c.kvHeads;
     const int unit = id / p.rows, row = id - unit * p.rows;     /* a pair or a tile, and a row of it */
@@ -119,24 +120,24 @@ attention_join_kernel(const JoinParams j)
         mx = newMax;
     }
     if (lane == 0) {
-        sh.stat[0][group][0] = mx;
-        sh.stat[0][group][1] = sum;
+        partStat[group][0] = mx;
+        partStat[group][1] = sum;
     }
-    *reinterpret_cast<f32x4 *>(&sh.acc[0][group][col]) = acc;
+    *reinterpret_cast<f32x4 *>(&partAcc[group][col]) = acc;
     __syncthreads();
     if (threadIdx.x < 32 && col < dh) {
-        float top = sh.stat[0][0][0];
+        float top = partStat[0][0];
 #pragma unroll
         for (int g = 1; g < 8; g++)
-            top = fmaxf(top, sh.stat[0][g][0]);
+            top = fmaxf(top, partStat[g][0]);
         const float shift = top == -INFINITY ? 0.f : top;
         float total = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int g = 0; g < 8; g++) {
-            const float f = __builtin_amdgcn_exp2f(sh.stat[0][g][0] - shift);
-            total += f * sh.stat[0][g][1];
-            o += *reinterpret_cast<const f32x4 *>(&sh.acc[0][g][col]) * f;
+            const float f = __builtin_amdgcn_exp2f(partStat[g][0] - shift);
+            total += f * partStat[g][1];
+            o += *reinterpret_cast<const f32x4 *>(&partAcc[g][col]) * f;
         }
         const float inv = total == 0.f ? 0.f : 1.f / total;
         typedef T vec __attribute__((ext_vector_type(4)));

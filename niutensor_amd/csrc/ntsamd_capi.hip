@@ -1033,7 +1033,7 @@ constexpr int CACHED_UNIT_HALF = 32, CACHED_UNIT_FLOAT = 16;
 
 int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool half, int prefix)
 {
-    const int unit = half ? CACHED_UNIT_HALF : CACHED_UNIT_FLOAT, qrMost = half ? 4 : 2;
+    const int unit = half ? CACHED_UNIT_HALF : CACHED_UNIT_FLOAT;
     const int kv = p.c.kvHeads, dh = p.c.dh, n = p.c.sequences;
     const long long rows = (long long)p.c.maxNew * p.per;           /* of one sequence and key head, at most */
     int cus = devID >= 0 && devID < MAX_DEVICES ? g_deviceCUs[devID].load(std::memory_order_relaxed) : 0;
@@ -1042,7 +1042,14 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     const long long slotRow = (long long)(dh + 2) * 4;              /* bytes of a partial row */
     const bool mayHold = tuning().splitK.load(std::memory_order_relaxed) != 1;
     const auto units = [unit](long long keys) { return (keys + unit - 1) / unit; };
-    const auto blocks_of = [](long long r) { return r <= 16 ? 1 : (r <= 32 ? 2 : 4); };
+    /* a tile of rows: up to 32 go to the kernel whose waves take keys of their own, half tiles of more rows to the one
+       that shares keys through LDS */
+    const auto tile_rows = [half](long long r) { return r <= 16 ? 16 : (r <= 32 || !half ? 32 : (r <= 64 ? 64 : 128)); };
+    const auto launch = [half, stream](const CachedParams & c, int tile, long long blocks) {
+        return tile > 32 ? launch_attention_cached_tiles(c, tile / 64, (int)blocks, stream)
+                         : launch_attention_cached(c, half, tile / 16, (int)blocks, stream);
+    };
+    const auto tile_kernel = [](int tile) { return tile > 32 ? "attention_cached_tiles_kernel" : "attention_cached_kernel"; };
     WorkHold work;
     int rc = 0;
     char text[160] = "";
@@ -1053,10 +1060,11 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     p.acc = p.stat = NULL;
     prefix = prefix < p.c.maxLength ? prefix : p.c.maxLength;
 
-    if (rows > 16 * qrMost) {
+    if (rows > 32) {
         /* many rows to a sequence: tiles of rows, their keys in one piece where the tiles fill the part */
         p.mode = CACHED_TILES;
-        p.rows = 16 * qrMost;
+        p.rows = tile_rows(rows);
+        const int keys = p.rows > 32 ? CACHED_TILE_KEYS : 4 * unit;      /* that a workgroup takes at a time */
         const long long perSeq = (rows + p.rows - 1) / p.rows;
         long long tiles = (long long)p.c.tokens * p.per / p.rows + n;
         if (!p.c.starts || n * perSeq < tiles)
@@ -1064,7 +1072,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         long long pieces = 1;
         if (mayHold && tiles * kv < 2 * cus) {
             pieces = (2 * cus + tiles * kv - 1) / (tiles * kv);
-            const long long most = (units(p.c.maxLength) + 15) / 16, fit = (long long)SPLIT_WORK_BYTES / (tiles * kv * p.rows * slotRow);
+            const long long most = (p.c.maxLength + 4 * keys - 1) / (4 * keys), fit = (long long)SPLIT_WORK_BYTES / (tiles * kv * p.rows * slotRow);
             pieces = pieces < most ? pieces : most;
             pieces = pieces < fit ? pieces : fit;
             if (pieces > 1) {
@@ -1083,11 +1091,11 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             p.acc = work.mem;
             p.stat = p.acc + tiles * kv * pieces * p.rows * dh;
         }
-        snprintf(g_plan, sizeof(g_plan), "attention_cached_kernel tiles=%lldx%d pieces=%lld%s", tiles, p.rows, pieces,
+        snprintf(g_plan, sizeof(g_plan), "%s tiles=%lldx%d pieces=%lld%s", tile_kernel(p.rows), tiles, p.rows, pieces,
                  pieces > 1 ? "+attention_join_kernel" : "");
         if (g_planOnly)
             return NTSAMD_OK;
-        rc = launch_attention_cached(p, half, qrMost, (int)(tiles * kv * pieces), stream);
+        rc = launch(p, p.rows, tiles * kv * pieces);
         if (rc == 0 && pieces > 1) {
             JoinParams j;
             memset(&j, 0, sizeof(j));
@@ -1096,10 +1104,10 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         }
     }
     else {
-        const int qr = blocks_of(rows);
+        const int tile = tile_rows(rows);
         p.rows = (int)rows;
         const long long room = (long long)SPLIT_WORK_BYTES / slotRow;       /* partial rows that fit */
-        const bool shared = prefix >= 4 * unit && n > 1 && mayHold && 256LL * kv <= room;
+        const bool shared = prefix >= 4 * unit && n > 1 && mayHold && 512LL * kv <= room;
         const long long own = p.c.maxLength - (shared ? prefix : 0);
         bool flat = mayHold && units(own) > 8;
         if (shared || flat) {
@@ -1131,14 +1139,14 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             if (withPrefix) {
                 CachedParams s = o;
                 const long long all = o.seqs * rows;
-                const int sqr = all <= 16 ? 1 : (all <= 32 || qrMost == 2 ? 2 : 4);
                 s.mode = CACHED_TILES;
                 s.prefix = prefix;
-                s.rows = 16 * sqr;
+                s.rows = tile_rows(all);
                 s.tiles = (int)((all + s.rows - 1) / s.rows);
                 const long long slots = (long long)s.tiles * kv;
                 long long pieces = (2 * cus + slots - 1) / slots;
-                const long long most = (units(prefix) + 3) / 4, fit = room / 2 / (slots * s.rows);
+                const int keys = s.rows > 32 ? CACHED_TILE_KEYS : 4 * unit;
+                const long long most = (prefix + keys - 1) / keys, fit = room / 2 / (slots * s.rows);
                 pieces = pieces < most ? pieces : most;
                 pieces = pieces < fit ? pieces : fit;
                 if (pieces < 1)
@@ -1151,9 +1159,9 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 j.preStat = s.stat;
                 j.prePieces = s.groups;
                 j.preRows = s.rows;
-                snprintf(text, sizeof(text), "attention_cached_kernel prefix tiles=%dx%d pieces=%lld+", s.tiles, s.rows, pieces);
+                snprintf(text, sizeof(text), "%s prefix tiles=%dx%d pieces=%lld+", tile_kernel(s.rows), s.tiles, s.rows, pieces);
                 if (!g_planOnly)
-                    rc = launch_attention_cached(s, half, sqr, (int)(slots * pieces), stream);
+                    rc = launch(s, s.rows, slots * pieces);
             }
             o.first = prefix;
             long long blocks = pairs;
@@ -1175,12 +1183,12 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 o.acc = work.mem + used * (dh + 2);
                 o.stat = o.acc + slots * rows * dh;
             }
-            snprintf(g_plan, sizeof(g_plan), "%sattention_cached_kernel rows=%d %s=%lld%s", text, 16 * qr,
+            snprintf(g_plan, sizeof(g_plan), "%sattention_cached_kernel rows=%d %s=%lld%s", text, tile,
                      o.mode == CACHED_FLAT ? "flat" : "whole", blocks, o.acc ? "+attention_join_kernel" : "");
             if (g_planOnly)
                 return NTSAMD_OK;
             if (rc == 0)
-                rc = launch_attention_cached(o, half, qr, (int)blocks, stream);
+                rc = launch(o, tile, blocks);
             if (rc == 0 && o.acc) {
                 j.p = o;
                 rc = launch_attention_join(j, half, (int)(pairs * rows), stream);
