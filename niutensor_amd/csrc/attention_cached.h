@@ -13,7 +13,7 @@ struct CachedScan {
     int found;
 };
 
-/* units of keys of one (sequence, key head) pair of a CACHED_FLAT launch: at least one where there are tokens to answer */
+/* units of keys of one (sequence, key head) pair: at least one where there are tokens to answer */
 template <int UK>
 __device__ __forceinline__ int units_of(const CachedParams & p, const CacheSequence & s)
 {
@@ -58,16 +58,16 @@ __device__ __forceinline__ SequenceScan scan_sequences(int count, CachedScan & s
     return r;
 }
 
-/* the sequence of a launch in which place `at` of the sum falls, and the sum before it; -1 past the end */
+/* the sequence of a launch in which place `at` of the sum (of its low half) falls, and the sum before it; -1 past the end */
 template <typename W>
-__device__ __forceinline__ int find_sequence(const SequenceScan & r, long long at, long long & before, CachedScan & sh, W weight)
+__device__ __forceinline__ int find_sequence(const SequenceScan & r, int at, long long & before, CachedScan & sh, W weight)
 {
-    if (at >= r.total)
+    if (at >= (int)r.total)
         return -1;
-    if (at >= r.before && at < r.before + r.sum) {
+    if (at >= (int)r.before && at < (int)r.before + (int)r.sum) {
         long long b = r.before;
         int i = r.from;
-        for (long long w = weight(i); at >= b + w; w = weight(i)) {
+        for (long long w = weight(i); i + 1 < r.to && at >= (int)b + (int)w; w = weight(i)) {
             b += w;
             i++;
         }
@@ -80,21 +80,31 @@ __device__ __forceinline__ int find_sequence(const SequenceScan & r, long long a
     return i;
 }
 
-/* CACHED_FLAT: unit x of the whole launch belongs to workgroup owner(x), whose units are start(w) .. start(w + 1) - 1 */
-struct FlatPlan {
+/* CACHED_PIECES: every (sequence, key head) pair is cut into pieces of at most `most` units, `most` such that all units
+   together make about p.groups pieces: at most p.groups + the number of pairs, and at most 2 p.groups of pairs that have more
+   than one. Both sums over the sequences travel in one: pieces in the low half, pieces of cut pairs in the high one. */
+struct PiecePlan {
+    long long most;
     SequenceScan scan;
-    int groups;
-    __device__ __forceinline__ long long start(int w) const { return scan.total * w / groups; }
-    __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * groups - 1) / scan.total); }
 };
 
-/* a workgroup's four waves take a unit each at a time: no more workgroups than whole rounds */
 template <int UK>
-__device__ __forceinline__ FlatPlan flat_plan(const CachedParams & p, CachedScan & sh)
+__device__ __forceinline__ long long pieces_of(const CachedParams & p, int i, long long most)
 {
-    FlatPlan f;
-    f.scan = scan_sequences(p.seqs, sh, [&](int i) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)) * p.c.kvHeads; });
-    f.groups = (int)min((long long)p.groups, (f.scan.total + 3) / 4);
+    const long long n = (units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)) + most - 1) / most;
+    return n * p.c.kvHeads + (n > 1 ? (n * p.c.kvHeads) << 32 : 0);
+}
+
+template <int UK>
+__device__ __forceinline__ PiecePlan piece_plan(const CachedParams & p, CachedScan & sh)
+{
+    PiecePlan f;
+    const SequenceScan units = scan_sequences(p.seqs, sh, [&](int i) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)); });
+    /* whole rounds of the four waves, which take a unit each at a time */
+    const long long total = units.total * p.c.kvHeads;
+    f.most = ((total + p.groups - 1) / p.groups + 3) / 4 * 4;
+    __syncthreads();
+    f.scan = scan_sequences(p.seqs, sh, [&](int i) { return pieces_of<UK>(p, i, f.most); });
     return f;
 }
 

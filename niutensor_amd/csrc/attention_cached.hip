@@ -344,35 +344,31 @@ attention_cached_kernel(const CachedParams p)
         if (sg.rows > 0)
             attend<T, DHM, QR>(p, sg, sh);
     }
-    else if (p.mode == CACHED_FLAT) {
-        const FlatPlan f = flat_plan<UK>(p, sh.scan);
-        if (id >= f.groups)
-            return;
-        const long long begin = f.start(id), end = f.start(id + 1);
+    else if (p.mode == CACHED_PIECES) {
+        const PiecePlan f = piece_plan<UK>(p, sh.scan);
         long long before;
-        int i = find_sequence(f.scan, begin, before, sh.scan,
-                              [&](int n) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + n)) * p.c.kvHeads; });
-        for (long long at = begin; at < end;) {
-            sg.seq = p.seq0 + i;
-            sg.s = cache_sequence(p.c, sg.seq);
-            const int units = units_of<UK>(p, sg.s);
-            for (; at < end && at < before + (long long)units * p.c.kvHeads;) {
-                const long long in = at - before;
-                sg.head = (int)(in / units);
-                sg.u0 = (int)(in - (long long)sg.head * units);
-                sg.u1 = (int)min((long long)units, sg.u0 + (end - at));
-                sg.row0 = 0;
-                sg.rows = sg.s.fresh * p.per;
-                if (sg.u0 == 0 && sg.u1 == units)
-                    sg.slot = p.first > 0 ? 2 * p.groups + i * p.c.kvHeads + sg.head : -1;
-                else
-                    sg.slot = 2 * id + (at == begin ? 0 : 1);
-                attend<T, DHM, QR>(p, sg, sh);
-                at += sg.u1 - sg.u0;
-            }
-            before += (long long)units * p.c.kvHeads;
-            i++;
+        const int i = find_sequence(f.scan, id, before, sh.scan, [&](int n) { return pieces_of<UK>(p, n, f.most); });
+        if (i < 0)
+            return;
+        sg.seq = p.seq0 + i;
+        sg.s = cache_sequence(p.c, sg.seq);
+        const int units = units_of<UK>(p, sg.s), pieces = (int)((units + f.most - 1) / f.most);
+        /* the key heads of a piece side by side: their rows may be neighbours in memory */
+        const int in = id - (int)before, piece = in / p.c.kvHeads;
+        sg.head = in - piece * p.c.kvHeads;
+        sg.row0 = 0;
+        sg.rows = sg.s.fresh * p.per;
+        sg.u0 = (int)((long long)units * piece / pieces);
+        sg.u1 = (int)((long long)units * (piece + 1) / pieces);
+        /* slots of cut pairs are numbered through; behind a prefix the others have one each after those */
+        const int pair = i * p.c.kvHeads + sg.head;
+        const int slot0 = pieces > 1 ? (int)(before >> 32) + sg.head * pieces : (p.first > 0 ? 2 * p.groups + pair : -1);
+        sg.slot = slot0 < 0 ? -1 : slot0 + piece;
+        if (piece == 0 && threadIdx.x == 0) {
+            p.slots[2 * pair] = slot0;
+            p.slots[2 * pair + 1] = slot0 < 0 ? 0 : pieces;
         }
+        attend<T, DHM, QR>(p, sg, sh);
     }
     else {
         if (!tile_segment<TR, UK>(p, sh.scan, id, sg))

@@ -3,8 +3,7 @@
  * a_i with the maximum m_i and the sum l_i of its softmax (base 2), give
  *   out = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i,   M = max_i m_i.
  * One workgroup per row: lanes of 4 columns, eight groups of them, which take the pieces in turn, in the order of the
- * keys, and meet in LDS in a fixed order, so results are the same bits on every run. Which pieces a row has is
- * worked out from the lengths as the first kernel did it: nothing about them is stored.
+ * keys, and meet in LDS in a fixed order, so results are the same bits on every run.
  */
 #include "gemm_common.h"
 #include "gemm_f16.h"       /* half_t */
@@ -14,7 +13,7 @@ namespace ntsamd {
 
 namespace {
 
-template <typename T, int UK>
+template <typename T>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(const JoinParams j)
 {
@@ -25,8 +24,7 @@ attention_join_kernel(const JoinParams j)
     const int unit = id / p.rows, row = id - unit * p.rows;     /* a pair or a tile, and a row of it */
     int head, inSeq;                    /* key head; the row among its sequence's */
     CacheSequence s;
-    /* the pieces: slot0, then step apart from slot1 on */
-    int pieces = 1, slot0, slot1 = 0, step = 0;
+    int pieces = 1, slot0 = unit;
     if (p.mode == CACHED_TILES) {
         const int tile = unit / kv;
         head = unit - tile * kv;
@@ -40,40 +38,17 @@ attention_join_kernel(const JoinParams j)
         inSeq = (tile - (int)before) * p.rows + row;
         pieces = p.groups;
         slot0 = unit * p.groups;
-        slot1 = slot0 + 1;
-        step = 1;
     }
     else {
         const int i = unit / kv;
         head = unit - i * kv;
         s = cache_sequence(p.c, p.seq0 + i);
         inSeq = row;
-        slot0 = unit;
-        if (p.mode == CACHED_FLAT) {
-            const FlatPlan f = flat_plan<UK>(p, sh);
-            if (i >= f.scan.from && i < f.scan.to) {
-                long long b = f.scan.before;
-                for (int n = f.scan.from; n < i; n++)
-                    b += (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + n)) * kv;
-                sh.before = b;
-            }
-            __syncthreads();
-            const int units = units_of<UK>(p, s);
-            if (units == 0)
-                return;
-            const long long begin = sh.before + (long long)head * units;
-            const int first = f.owner(begin), last = f.owner(begin + units - 1);
-            pieces = last - first + 1;
-            if (pieces == 1) {
-                if (p.first == 0)
-                    return;             /* one workgroup had them all: the result stands in out */
-                slot0 = 2 * p.groups + unit;
-            }
-            else {
-                slot0 = 2 * first + (f.start(first) == begin ? 0 : 1);
-                slot1 = 2 * (first + 1);
-                step = 2;
-            }
+        if (p.mode == CACHED_PIECES && s.fresh > 0) {
+            slot0 = p.slots[2 * unit];
+            pieces = p.slots[2 * unit + 1];
+            if (pieces == 0)
+                return;                 /* one workgroup had all keys: the result stands in out */
         }
     }
     if (inSeq >= s.fresh * p.per)
@@ -97,26 +72,35 @@ attention_join_kernel(const JoinParams j)
     const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, col = 4 * lane;
     float mx = -INFINITY, sum = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int i = group; i < pre + pieces; i += 8) {
-        const float * a;
-        const float * st;
-        if (i < pre) {
-            const long long at = (long long)(preSlot + i) * j.preRows + preRow;
-            a = j.preAcc + at * dh;
-            st = j.preStat + 2 * at;
+    constexpr int AHEAD = 4;            /* pieces of a group in flight */
+    for (int i0 = group; i0 < pre + pieces; i0 += 8 * AHEAD) {
+        float m[AHEAD], l[AHEAD];
+        f32x4 x[AHEAD];
+        float newMax = mx;
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            const int i = min(i0 + 8 * e, pre + pieces - 1);
+            const bool own = i >= pre;
+            const long long at = own ? (long long)(slot0 + i - pre) * p.rows + row : (long long)(preSlot + i) * j.preRows + preRow;
+            const float * st = (own ? p.stat : j.preStat) + 2 * at;
+            const bool there = i0 + 8 * e < pre + pieces;
+            m[e] = there ? st[0] : -INFINITY;
+            l[e] = there ? st[1] : 0.f;
+            x[e] = there && col < dh ? *reinterpret_cast<const f32x4 *>((own ? p.acc : j.preAcc) + at * dh + col) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        else {
-            const long long at = (long long)(i == pre ? slot0 : slot1 + (i - pre - 1) * step) * p.rows + row;
-            a = p.acc + at * dh;
-            st = p.stat + 2 * at;
-        }
-        const float m = st[0], l = st[1];
-        const f32x4 x = col < dh ? *reinterpret_cast<const f32x4 *>(a + col) : f32x4{0.f, 0.f, 0.f, 0.f};
-        const float newMax = fmaxf(mx, m);
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++)
+            newMax = fmaxf(newMax, m[e]);
         const float shift = newMax == -INFINITY ? 0.f : newMax;
-        const float f0 = __builtin_amdgcn_exp2f(mx - shift), f1 = __builtin_amdgcn_exp2f(m - shift);
-        sum = sum * f0 + l * f1;
-        acc = acc * f0 + x * f1;
+        const float f0 = __builtin_amdgcn_exp2f(mx - shift);
+        sum *= f0;
+        acc *= f0;
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            const float f = __builtin_amdgcn_exp2f(m[e] - shift);
+            sum += l[e] * f;
+            acc += x[e] * f;
+        }
         mx = newMax;
     }
     if (lane == 0) {
@@ -154,11 +138,10 @@ attention_join_kernel(const JoinParams j)
 
 int launch_attention_join(const JoinParams & j, bool half, int blocks, hipStream_t stream)
 {
-    /* UK: the unit of attention_cached_kernel for the type */
     if (half)
-        hipLaunchKernelGGL((attention_join_kernel<half_t, 32>), dim3((unsigned)blocks), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL((attention_join_kernel<half_t>), dim3((unsigned)blocks), dim3(256), 0, stream, j);
     else
-        hipLaunchKernelGGL((attention_join_kernel<float, 16>), dim3((unsigned)blocks), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL((attention_join_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, j);
     return (int)hipGetLastError();
 }
 

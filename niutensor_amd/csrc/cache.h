@@ -94,18 +94,19 @@ struct CachedParams {
     int first;                          /* positions before this one are another launch's (the shared prefix) */
     int prefix;                         /* > 0: this launch is the shared prefix of that many positions */
     int mode;                           /* CachedMode */
-    int groups;                         /* CACHED_FLAT: workgroups of the launch; CACHED_TILES: pieces of a tile's keys */
+    int groups;                         /* CACHED_PIECES: pieces aimed at; CACHED_TILES: pieces of a tile's keys */
     int tiles;                          /* CACHED_TILES: tiles launched (at least those that the batch can have) */
     int rows;                           /* rows of a slot */
     /* partial results: acc[slot][row][dh] and stat[slot][row][2] (maximum and sum, base 2); NULL: results go to out */
     float * acc;
     float * stat;
+    int * slots;                        /* CACHED_PIECES: first slot and number of pieces of every pair, for the join */
 };
 
 /* CACHED_WHOLE: a workgroup takes all keys of one (sequence, key head).
-   CACHED_FLAT: the keys of all (sequence, key head) pairs laid end to end and cut into equal pieces, one per workgroup.
+   CACHED_PIECES: the keys of every pair cut into pieces of about the same length, one workgroup each.
    CACHED_TILES: rows cut into tiles (several to a sequence), the keys of a tile into `groups` pieces. */
-enum CachedMode { CACHED_WHOLE = 0, CACHED_FLAT = 1, CACHED_TILES = 2 };
+enum CachedMode { CACHED_WHOLE = 0, CACHED_PIECES = 1, CACHED_TILES = 2 };
 
 int launch_cache_append(AppendParams p, bool half, hipStream_t stream);
 

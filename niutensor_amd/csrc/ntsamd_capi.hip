@@ -1167,24 +1167,26 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             long long blocks = pairs;
             o.mode = CACHED_WHOLE;
             if (flat) {
-                /* two workgroups to a CU, in rounds of a unit to a wave; their slots, and one for each pair behind a prefix */
-                const long long left = room - used - (withPrefix ? pairs * rows : 0);
-                long long groups = 2 * cus, need = (pairs * units(own) + 3) / 4;
-                groups = groups < need ? groups : need;
+                /* what is left holds 2 `groups` slots, one more for each pair behind a prefix, and two numbers for each pair */
+                const long long left = room - used - (withPrefix ? pairs * rows : 0) - (pairs * 8 + slotRow - 1) / slotRow;
+                long long groups = tuning().groupM.load() > 0 ? tuning().groupM.load() : 4 * cus;
                 groups = groups < left / (2 * rows) ? groups : left / (2 * rows);
-                if (groups >= 1) {
-                    o.mode = CACHED_FLAT;
+                if (groups >= cus / 2) {
+                    o.mode = CACHED_PIECES;
                     o.groups = (int)groups;
-                    blocks = groups;
+                    blocks = groups + pairs;
+                    const long long most = pairs * ((units(own) + 3) / 4);
+                    blocks = blocks < most ? blocks : most;
                 }
             }
-            if (withPrefix || o.mode == CACHED_FLAT) {
-                const long long slots = (o.mode == CACHED_FLAT ? 2 * blocks : 0) + (withPrefix ? pairs : 0);
+            if (withPrefix || o.mode == CACHED_PIECES) {
+                const long long slots = (o.mode == CACHED_PIECES ? 2LL * o.groups : 0) + (withPrefix ? pairs : 0);
                 o.acc = work.mem + used * (dh + 2);
                 o.stat = o.acc + slots * rows * dh;
+                o.slots = reinterpret_cast<int *>(o.stat + 2 * slots * rows);
             }
             snprintf(g_plan, sizeof(g_plan), "%sattention_cached_kernel rows=%d %s=%lld%s", text, tile,
-                     o.mode == CACHED_FLAT ? "flat" : "whole", blocks, o.acc ? "+attention_join_kernel" : "");
+                     o.mode == CACHED_PIECES ? "pieces" : "whole", blocks, o.acc ? "+attention_join_kernel" : "");
             if (g_planOnly)
                 return NTSAMD_OK;
             if (rc == 0)

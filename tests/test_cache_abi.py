@@ -128,9 +128,9 @@ def planning():
 def test_plans(planning):
     # short sequences: a workgroup takes a pair's keys alone, and nothing is joined
     assert attend(n=8, tokens=8, width=4) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 whole=16"
-    # long ones: keys laid end to end
+    # long ones: in pieces
     assert attend(n=8, tokens=8, width=512) == 0
-    assert re.fullmatch(r"attention_cached_kernel rows=16 flat=512\+attention_join_kernel", nt.last_plan())
+    assert re.fullmatch(r"attention_cached_kernel rows=16 pieces=\d+\+attention_join_kernel", nt.last_plan())
     nt.tuning_set("NTSAMD_SPLIT_K", 1)
     assert attend(n=8, tokens=8, width=512) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 whole=16"
     assert attend(n=8, tokens=8, width=512, prefix=1024) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 whole=16"
