@@ -84,15 +84,16 @@ __device__ __forceinline__ int find_sequence(const SequenceScan & r, int at, lon
    together make about p.groups pieces: at most p.groups + the number of pairs, and at most 2 p.groups of pairs that have more
    than one. Both sums over the sequences travel in one: pieces in the low half, pieces of cut pairs in the high one. */
 struct PiecePlan {
-    long long most;
+    int most;
     SequenceScan scan;
 };
 
 template <int UK>
-__device__ __forceinline__ long long pieces_of(const CachedParams & p, int i, long long most)
+__device__ __forceinline__ long long pieces_of(const CachedParams & p, int i, int most)
 {
-    const long long n = (units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)) + most - 1) / most;
-    return n * p.c.kvHeads + (n > 1 ? (n * p.c.kvHeads) << 32 : 0);
+    const unsigned n = ((unsigned)units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)) + most - 1) / (unsigned)most;
+    const long long all = (long long)n * p.c.kvHeads;
+    return all + (n > 1 ? all << 32 : 0);
 }
 
 template <int UK>
@@ -102,7 +103,8 @@ __device__ __forceinline__ PiecePlan piece_plan(const CachedParams & p, CachedSc
     const SequenceScan units = scan_sequences(p.seqs, sh, [&](int i) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)); });
     /* whole rounds of the four waves, which take a unit each at a time */
     const long long total = units.total * p.c.kvHeads;
-    f.most = ((total + p.groups - 1) / p.groups + 3) / 4 * 4;
+    const long long each = total >> 31 ? (total + p.groups - 1) / p.groups : ((unsigned)total + p.groups - 1) / (unsigned)p.groups;
+    f.most = (int)min((each + 3) & ~3ll, 0x7ffffffcll);
     __syncthreads();
     f.scan = scan_sequences(p.seqs, sh, [&](int i) { return pieces_of<UK>(p, i, f.most); });
     return f;
@@ -160,9 +162,9 @@ __device__ __forceinline__ bool tile_segment(const CachedParams & p, CachedScan 
     int keys = sg.s.length;
     if (p.causal && p.prefix == 0)
         keys -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
-    const int units = (max(keys - p.first, 0) + UK - 1) / UK;
-    sg.u0 = (int)((long long)units * piece / p.groups);
-    sg.u1 = (int)((long long)units * (piece + 1) / p.groups);
+    const int units = (max(keys - p.first, 0) + UK - 1) / UK, each = (units + p.groups - 1) / p.groups;
+    sg.u0 = min(each * piece, units);
+    sg.u1 = min(sg.u0 + each, units);
     return true;
 }
 
@@ -237,13 +239,38 @@ __device__ __forceinline__ void rows_seen(const CachedParams & p, const Segment 
     most = __builtin_amdgcn_readfirstlane(most);
 }
 
-/* where positions that do not exist and columns past dh are read from */
-static __device__ const float zero_row[4] = {0.f, 0.f, 0.f, 0.f};
+/* What the positions that do not exist read: a row of the widest head. */
+static __device__ __align__(16) const float zero_row[128] = {};
+
+/* Where a lane's key stands: the address of its row of k and of v, or of a row of zeros. Addresses and not pointers, so that
+   they can be handed from lane to lane and loaded from as what they are, global memory. */
+struct KeyPlace {
+    long long k, v;
+    bool there;
+};
+
+template <typename T>
+__device__ __forceinline__ KeyPlace key_place(const CacheParams & c, int head, int key, int page)
+{
+    KeyPlace x;
+    x.there = page >= 0 && page < c.pages;
+    const int r = key - divided(key, c.pageSize) * (int)c.pageSize.d;
+    const long long zero = (long long)reinterpret_cast<uintptr_t>(zero_row);
+    x.k = x.there ? (long long)reinterpret_cast<uintptr_t>(static_cast<const T *>(c.k) + page * c.kP + r * c.kR + head * c.kH) : zero;
+    x.v = x.there ? (long long)reinterpret_cast<uintptr_t>(static_cast<const T *>(c.v) + page * c.vP + r * c.vR + head * c.vH) : zero;
+    return x;
+}
 
 __device__ __forceinline__ long long lane_of(long long x, int source)
 {
     const int lo = __shfl((int)x, source), hi = __shfl((int)(x >> 32), source);
     return ((long long)hi << 32) | (unsigned)lo;
+}
+
+template <typename V>
+__device__ __forceinline__ V load_global(long long address)
+{
+    return *(const __attribute__((address_space(1))) V *)address;
 }
 
 int launch_attention_cached(const CachedParams & p, bool half, int qr, int blocks, hipStream_t stream);

@@ -113,40 +113,36 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
 
     /* ---- loading a unit ---- */
     const int * table = c.table + (long long)sg.seq * c.tablePages;
-    const char * kBase = reinterpret_cast<const char *>(static_cast<const T *>(c.k) + sg.head * c.kH);
-    const char * vBase = reinterpret_cast<const char *>(static_cast<const T *>(c.v) + sg.head * c.vH);
-    const char * zero = reinterpret_cast<const char *>(zero_row);
     const int myKey = lane & (U::UK - 1);
     auto page_of = [&](int u) {
         const int key = p.first + u * U::UK + myKey;
         return u < sg.u1 && key < seenMax ? table[divided(key, c.pageSize)] : -1;
     };
+    /* byte offsets of a lane's columns in a row. Columns past dh read the row's first: a key's meet zeros of q, a value's
+       end in columns of the result that are not stored */
+    int kCol[U::NT], vCol[U::NH];
+#pragma unroll
+    for (int t = 0; t < U::NT; t++)
+        kCol[t] = 64 * t + 16 * g < dh * (int)sizeof(T) ? 64 * t + 16 * g : 0;
+#pragma unroll
+    for (int h = 0; h < U::NH; h++)
+        vCol[h] = U::VC * (16 * h + m) < dh ? U::VC * (16 * h + m) * (int)sizeof(T) : 0;
     auto load = [&](int u, int page, UnitData<T, DHM> & d) {
-        const int key = p.first + u * U::UK + myKey;
-        const bool valid = page >= 0 && page < c.pages;
-        const int r = key - divided(key, c.pageSize) * (int)c.pageSize.d;
-        const long long kOff = valid ? (page * c.kP + r * c.kR) * (long long)sizeof(T) : -1;
-        const long long vOff = valid ? (page * c.vP + r * c.vR) * (long long)sizeof(T) : -1;
-        d.there = (unsigned)__ballot(valid) & ALL;
+        const KeyPlace at = key_place<T>(c, sg.head, p.first + u * U::UK + myKey, page);
+        d.there = (unsigned)__ballot(at.there) & ALL;
 #pragma unroll
         for (int j = 0; j < U::NJ; j++) {
-            const long long off = lane_of(kOff, 16 * j + m);
-            const char * row = kBase + off;
+            const long long row = lane_of(at.k, 16 * j + m);
 #pragma unroll
-            for (int t = 0; t < U::NT; t++) {
-                const int col = (64 * t + 16 * g) / (int)sizeof(T);
-                d.k[j][t] = *reinterpret_cast<const typename U::KPiece *>(off >= 0 && col < dh ? row + 64 * t + 16 * g : zero);
-            }
+            for (int t = 0; t < U::NT; t++)
+                d.k[j][t] = load_global<typename U::KPiece>(row + kCol[t]);
         }
 #pragma unroll
         for (int e = 0; e < U::NV; e++) {
-            const long long off = lane_of(vOff, 16 * (e >> 2) + 4 * g + (e & 3));
-            const char * row = vBase + off;
+            const long long row = lane_of(at.v, 16 * (e >> 2) + 4 * g + (e & 3));
 #pragma unroll
-            for (int h = 0; h < U::NH; h++) {
-                const int col = U::VC * (16 * h + m);
-                d.v[e][h] = *reinterpret_cast<const typename U::VPiece *>(off >= 0 && col < dh ? row + col * (int)sizeof(T) : zero);
-            }
+            for (int h = 0; h < U::NH; h++)
+                d.v[e][h] = load_global<typename U::VPiece>(row + vCol[h]);
         }
     };
 
@@ -323,6 +319,36 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     }
 }
 
+/* CACHED_PIECES: the segment of workgroup `id`; false: it has none */
+template <int UK>
+__device__ __forceinline__ bool piece_segment(const CachedParams & p, CachedScan & sh, int id, Segment & sg)
+{
+    const PiecePlan f = piece_plan<UK>(p, sh);
+    long long before;
+    const int i = find_sequence(f.scan, id, before, sh, [&](int n) { return pieces_of<UK>(p, n, f.most); });
+    if (i < 0)
+        return false;
+    sg.seq = p.seq0 + i;
+    sg.s = cache_sequence(p.c, sg.seq);
+    const int units = units_of<UK>(p, sg.s), pieces = (int)(((unsigned)units + f.most - 1) / (unsigned)f.most);
+    /* the key heads of a piece side by side: their rows may be neighbours in memory */
+    const int in = id - (int)before, piece = in / p.c.kvHeads;
+    sg.head = in - piece * p.c.kvHeads;
+    sg.row0 = 0;
+    sg.rows = sg.s.fresh * p.per;
+    sg.u0 = piece * f.most;
+    sg.u1 = min(sg.u0 + f.most, units);
+    /* slots of cut pairs are numbered through; behind a prefix the others have one each after those */
+    const int pair = i * p.c.kvHeads + sg.head;
+    const int slot0 = pieces > 1 ? (int)(before >> 32) + sg.head * pieces : (p.first > 0 ? 2 * p.groups + pair : -1);
+    sg.slot = slot0 < 0 ? -1 : slot0 + piece;
+    if (piece == 0 && threadIdx.x == 0) {
+        p.slots[2 * pair] = slot0;
+        p.slots[2 * pair + 1] = slot0 < 0 ? 0 : pieces;
+    }
+    return true;
+}
+
 template <typename T, int DHM, int QR>
 __global__ void __launch_bounds__(256, QR == 2 && DHM == 128 ? 1 : 2)
 attention_cached_kernel(const CachedParams p)
@@ -331,7 +357,15 @@ attention_cached_kernel(const CachedParams p)
     __shared__ CachedShared sh;
     const int id = (int)blockIdx.x;
     Segment sg;
-    if (p.mode == CACHED_WHOLE) {
+    if (p.mode == CACHED_TILES) {
+        if (!tile_segment<TR, UK>(p, sh.scan, id, sg))
+            return;
+    }
+    else if (p.mode == CACHED_PIECES) {
+        if (!piece_segment<UK>(p, sh.scan, id, sg))
+            return;
+    }
+    else {
         const int i = id / p.c.kvHeads;
         sg.head = id - i * p.c.kvHeads;
         sg.seq = p.seq0 + i;
@@ -341,40 +375,10 @@ attention_cached_kernel(const CachedParams p)
         sg.u0 = 0;
         sg.u1 = (max(sg.s.length - p.first, 0) + UK - 1) / UK;
         sg.slot = p.acc ? id : -1;
-        if (sg.rows > 0)
-            attend<T, DHM, QR>(p, sg, sh);
-    }
-    else if (p.mode == CACHED_PIECES) {
-        const PiecePlan f = piece_plan<UK>(p, sh.scan);
-        long long before;
-        const int i = find_sequence(f.scan, id, before, sh.scan, [&](int n) { return pieces_of<UK>(p, n, f.most); });
-        if (i < 0)
+        if (sg.rows == 0)
             return;
-        sg.seq = p.seq0 + i;
-        sg.s = cache_sequence(p.c, sg.seq);
-        const int units = units_of<UK>(p, sg.s), pieces = (int)((units + f.most - 1) / f.most);
-        /* the key heads of a piece side by side: their rows may be neighbours in memory */
-        const int in = id - (int)before, piece = in / p.c.kvHeads;
-        sg.head = in - piece * p.c.kvHeads;
-        sg.row0 = 0;
-        sg.rows = sg.s.fresh * p.per;
-        sg.u0 = (int)((long long)units * piece / pieces);
-        sg.u1 = (int)((long long)units * (piece + 1) / pieces);
-        /* slots of cut pairs are numbered through; behind a prefix the others have one each after those */
-        const int pair = i * p.c.kvHeads + sg.head;
-        const int slot0 = pieces > 1 ? (int)(before >> 32) + sg.head * pieces : (p.first > 0 ? 2 * p.groups + pair : -1);
-        sg.slot = slot0 < 0 ? -1 : slot0 + piece;
-        if (piece == 0 && threadIdx.x == 0) {
-            p.slots[2 * pair] = slot0;
-            p.slots[2 * pair + 1] = slot0 < 0 ? 0 : pieces;
-        }
-        attend<T, DHM, QR>(p, sg, sh);
     }
-    else {
-        if (!tile_segment<TR, UK>(p, sh.scan, id, sg))
-            return;
-        attend<T, DHM, QR>(p, sg, sh);
-    }
+    attend<T, DHM, QR>(p, sg, sh);
 }
 
 template <typename T, int DHM>

@@ -51,9 +51,6 @@ attention_cached_tiles_kernel(const CachedParams p)
 
     /* ---- where the keys of a block stand: lane l looks after key l ---- */
     const int * table = c.table + (long long)sg.seq * c.tablePages;
-    const half_t * kBase = static_cast<const half_t *>(c.k) + sg.head * c.kH;
-    const half_t * vBase = static_cast<const half_t *>(c.v) + sg.head * c.vH;
-    const half_t * zero = reinterpret_cast<const half_t *>(zero_row);
     int keyEnd = sg.s.length;                /* the keys that any row of the tile sees */
     if (p.causal && p.prefix == 0)
         keyEnd -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
@@ -65,26 +62,20 @@ attention_cached_tiles_kernel(const CachedParams p)
     const int sLds = sr0 * PITCH + sc * 2;
     f16x8 kreg[LOADS], vreg[LOADS];
     unsigned long long there = 0;            /* which keys of the block being fetched exist */
-    long long vOff;
+    long long vRow = 0;
+    const int col = sc < dh ? 2 * sc : 0;    /* columns past dh: the row's first, which meet zeros of q or are not stored */
     auto load_k = [&](int u, int page) {
-        const int key = p.first + u * KB + lane;
-        const bool valid = page >= 0 && page < c.pages;
-        const int r = key - divided(key, c.pageSize) * (int)c.pageSize.d;
-        const long long kOff = valid ? page * c.kP + r * c.kR : -1;
-        vOff = valid ? page * c.vP + r * c.vR : -1;
-        there = __ballot(valid);
+        const KeyPlace at = key_place<half_t>(c, sg.head, p.first + u * KB + lane, page);
+        vRow = at.v;
+        there = __ballot(at.there);
 #pragma unroll
-        for (int s = 0; s < LOADS; s++) {
-            const long long off = lane_of(kOff, sr0 + s * RSTEP);
-            kreg[s] = *reinterpret_cast<const f16x8 *>(off >= 0 && sc < dh ? kBase + off + sc : zero);
-        }
+        for (int s = 0; s < LOADS; s++)
+            kreg[s] = load_global<f16x8>(lane_of(at.k, sr0 + s * RSTEP) + col);
     };
     auto load_v = [&]() {
 #pragma unroll
-        for (int s = 0; s < LOADS; s++) {
-            const long long off = lane_of(vOff, sr0 + s * RSTEP);
-            vreg[s] = *reinterpret_cast<const f16x8 *>(off >= 0 && sc < dh ? vBase + off + sc : zero);
-        }
+        for (int s = 0; s < LOADS; s++)
+            vreg[s] = load_global<f16x8>(lane_of(vRow, sr0 + s * RSTEP) + col);
     };
     int page = page_of(sg.u0);
     load_k(sg.u0, page);
