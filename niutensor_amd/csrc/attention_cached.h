@@ -239,6 +239,16 @@ __device__ __forceinline__ void rows_seen(const CachedParams & p, const Segment 
     most = __builtin_amdgcn_readfirstlane(most);
 }
 
+/* The softmax of a row runs on raw scores s and the base-2 scale of p: 2^(s scale2 - shift). Scores are multiplied by |scale|
+   (queries take its sign), at least by what leaves hidden scores at minus infinity. `shift` follows the row's maximum only
+   where that has grown by more than 2^RISE: until then probabilities are up to 2^RISE, which half holds with the same relative
+   precision, and sums and results need no rescaling (at most one block in a few has a row that does). */
+constexpr float CACHED_RISE = 8.f;
+__device__ __forceinline__ float score_scale(const CachedParams & p)
+{
+    return fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-37f);
+}
+
 /* What the positions that do not exist read: a row of the widest head. */
 static __device__ __align__(16) const float zero_row[128] = {};
 

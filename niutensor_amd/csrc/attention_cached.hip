@@ -84,7 +84,6 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
 {
     typedef Unit<T, DHM> U;
     constexpr int ND = DHM / 16;
-    constexpr float LOG2E = 1.4426950408889634f;
     constexpr unsigned ALL = U::UK == 32 ? 0xffffffffu : 0xffffu;
     const CacheParams & c = p.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -108,6 +107,8 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
             const int col = 4 * W * t4 + W * g;
             typename U::KPiece z = {};
             qf[q][t4] = there && col < dh ? *reinterpret_cast<const typename U::KPiece *>(qr + col) : z;
+            if (p.scale < 0.f)
+                qf[q][t4] = -qf[q][t4];
         }
     }
 
@@ -156,14 +157,13 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
         rowMax[q] = -INFINITY;
         rowSum[q] = 0.f;
     }
-    const float scale2 = p.scale * LOG2E;
+    const float scale2 = score_scale(p);
 
     UnitData<T, DHM> next;
     int u = sg.u0 + wave;
-    int page = page_of(u);
     if (u < sg.u1)
-        load(u, page, next);
-    page = page_of(u + 4);
+        load(u, page_of(u), next);
+    int page = page_of(u + 4);
     for (; u < sg.u1; u += 4) {
         const UnitData<T, DHM> d = next;
         if (u + 4 < sg.u1)
@@ -197,9 +197,6 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
         T pr[QR][U::NJ][4];                             /* the probabilities as the second product's operand */
 #pragma unroll
         for (int q = 0; q < QR; q++) {
-#pragma unroll
-            for (int j = 0; j < U::NJ; j++)
-                s[q][j] *= scale2;
             if (cut) {
 #pragma unroll
                 for (int j = 0; j < U::NJ; j++)
@@ -216,23 +213,25 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     mx = fmaxf(mx, s[q][j][r]);
-            const float newMax = fmaxf(rowMax[q], lane_groups_max(mx));
-            const float shift = newMax == -INFINITY ? 0.f : newMax;
-            const float corr = __builtin_amdgcn_exp2f(rowMax[q] - shift);
-            float sum = 0.f;
+            mx = lane_groups_max(mx) * scale2;
+            if (__any(mx > rowMax[q] + CACHED_RISE)) {
+                const float newMax = fmaxf(rowMax[q], mx);
+                const float corr = __builtin_amdgcn_exp2f(rowMax[q] - (newMax == -INFINITY ? 0.f : newMax));
+                rowSum[q] *= corr;
+                rowMax[q] = newMax;
+#pragma unroll
+                for (int e = 0; e < ND; e++)
+                    accO[q][e] *= corr;
+            }
+            const float shift = rowMax[q] == -INFINITY ? 0.f : rowMax[q];
 #pragma unroll
             for (int j = 0; j < U::NJ; j++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float e = __builtin_amdgcn_exp2f(s[q][j][r] - shift);
-                    sum += e;
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[q][j][r], scale2, -shift));
+                    rowSum[q] += e;                     /* this lane's keys only: the lanes of a row meet at the end */
                     pr[q][j][r] = (T)e;
                 }
-            rowSum[q] = rowSum[q] * corr + sum;         /* this lane's keys only: the lanes of a row meet at the end */
-            rowMax[q] = newMax;
-#pragma unroll
-            for (int e = 0; e < ND; e++)
-                accO[q][e] *= corr;
         }
 
         /* ---- O^T += V^T P^T ---- */

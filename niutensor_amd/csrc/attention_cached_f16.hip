@@ -21,7 +21,7 @@ namespace ntsamd {
 namespace {
 
 template <int DHM, int QR>
-__global__ void __launch_bounds__(256, QR == 2 && DHM <= 64 ? 3 : 2)
+__global__ void __launch_bounds__(256, 2)
 attention_cached_tiles_kernel(const CachedParams p)
 {
     constexpr int KB = CACHED_TILE_KEYS, TR = 64 * QR;
@@ -30,7 +30,6 @@ attention_cached_tiles_kernel(const CachedParams p)
     constexpr int NT = DHM / 32, ND = DHM / 16, NJ = KB / 16;
     constexpr int TPR = DHM / 8;             /* threads per row when staging */
     constexpr int RSTEP = 256 / TPR, LOADS = KB / RSTEP;
-    constexpr float LOG2E = 1.4426950408889634f;
 
     __shared__ __attribute__((aligned(16))) char Ks[KB * PITCH];
     __shared__ __attribute__((aligned(16))) char Vs[KB * PITCH];
@@ -79,6 +78,7 @@ attention_cached_tiles_kernel(const CachedParams p)
     };
     int page = page_of(sg.u0);
     load_k(sg.u0, page);
+    load_v();
     page = page_of(sg.u0 + 1);
 
     /* ---- Q fragments ---- */
@@ -95,6 +95,8 @@ attention_cached_tiles_kernel(const CachedParams p)
             const int col = 32 * t4 + 8 * g;
             const f16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
             qf[q][t4] = has && col < dh ? *reinterpret_cast<const f16x8 *>(qr + col) : z;
+            if (p.scale < 0.f)
+                qf[q][t4] = -qf[q][t4];
         }
     }
 
@@ -108,21 +110,18 @@ attention_cached_tiles_kernel(const CachedParams p)
         rowMax[q] = -INFINITY;
         rowSum[q] = 0.f;
     }
-    const float scale2 = p.scale * LOG2E;
+    const float scale2 = score_scale(p);
     /* where this lane points for the transposing reads: row 4 g + (m / 4) of a 16-key block, columns 4 (m % 4) .. + 3 */
     const int trOff = (4 * g + (m >> 2)) * PITCH + (m & 3) * 8;
 
     for (int u = sg.u0; u < sg.u1; u++) {
-        const bool more = u + 1 < sg.u1;
         const int key0 = p.first + u * KB;
         const unsigned long long exist = there;
 #pragma unroll
         for (int s = 0; s < LOADS; s++)
             *reinterpret_cast<f16x8 *>(&Ks[sLds + s * RSTEP * PITCH]) = kreg[s];
-        load_v();                            /* of this block: they are due after the first product */
         __syncthreads();
-        if (more)
-            load_k(u + 1, page);
+        load_k(u + 1, page);                 /* past the end: rows of zeros */
         page = page_of(u + 2);
 
         /* ---- S^T = K Q^T ---- */
@@ -144,12 +143,11 @@ attention_cached_tiles_kernel(const CachedParams p)
 
         /* ---- running softmax of the lane's rows ---- */
         f16x4 pf[QR][NJ];
+        float top[QR];
+        bool risen = false;
         const bool cut = exist != ~0ull || key0 + KB > seenMin;
 #pragma unroll
         for (int q = 0; q < QR; q++) {
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-                accS[q][j] *= scale2;
             if (cut) {
 #pragma unroll
                 for (int j = 0; j < NJ; j++)
@@ -166,29 +164,39 @@ attention_cached_tiles_kernel(const CachedParams p)
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     mx = fmaxf(mx, accS[q][j][r]);
-            const float newMax = fmaxf(rowMax[q], lane_groups_max(mx));
-            const float shift = newMax == -INFINITY ? 0.f : newMax;
-            const float corr = __builtin_amdgcn_exp2f(rowMax[q] - shift);
-            float sum = 0.f;
+            top[q] = lane_groups_max(mx) * scale2;
+            risen = risen || top[q] > rowMax[q] + CACHED_RISE;
+        }
+        if (__any(risen)) {
+#pragma unroll
+            for (int q = 0; q < QR; q++) {
+                const float newMax = fmaxf(rowMax[q], top[q]);
+                const float corr = __builtin_amdgcn_exp2f(rowMax[q] - (newMax == -INFINITY ? 0.f : newMax));
+                rowSum[q] *= corr;
+                rowMax[q] = newMax;
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+                    accO[q][d] *= corr;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < QR; q++) {
+            const float shift = rowMax[q] == -INFINITY ? 0.f : rowMax[q];
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float e = __builtin_amdgcn_exp2f(accS[q][j][r] - shift);
-                    sum += e;
+                    const float e = __builtin_amdgcn_exp2f(fmaf(accS[q][j][r], scale2, -shift));
+                    rowSum[q] += e;                      /* this lane's keys only: the four lanes of a row meet at the end */
                     pf[q][j][r] = (half_t)e;
                 }
-            rowSum[q] = rowSum[q] * corr + sum;          /* this lane's keys only: the four lanes of a row meet at the end */
-            rowMax[q] = newMax;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-                accO[q][d] *= corr;
         }
 
 #pragma unroll
         for (int s = 0; s < LOADS; s++)
             *reinterpret_cast<f16x8 *>(&Vs[sLds + s * RSTEP * PITCH]) = vreg[s];
         __syncthreads();
+        load_v();
 
         /* ---- O^T += V^T P^T, 32 keys per MFMA: its k index 8 g + e stands for key 4 g + e of the first 16-key block of a
            pair for e < 4 and for key 4 g + e - 4 of the second for e >= 4 ---- */
