@@ -114,10 +114,29 @@ __device__ __forceinline__ PiecePlan piece_plan(const CachedParams & p, CachedSc
 struct Segment {
     CacheSequence s;
     int seq, head;                      /* table row, key head */
-    int row0, rows;                     /* first row of the tile, rows the sequence has */
+    int row0, rows;                     /* first row of the tile, rows the sequence has (0: nothing to do) */
+    int keys;                           /* positions that any row of the tile sees */
     int u0, u1;                         /* units, from p.first on */
     int slot;                           /* where the partial result goes, -1: the result goes to out */
 };
+
+/* The same for all lanes: in scalar registers. (Loaded by lanes, kept by lanes: the table's address alone would be
+   spilled, and a reload inside the loop waits for every row in flight.) */
+__device__ __forceinline__ Segment uniform(Segment sg)
+{
+    sg.s.start = __builtin_amdgcn_readfirstlane(sg.s.start);
+    sg.s.fresh = __builtin_amdgcn_readfirstlane(sg.s.fresh);
+    sg.s.length = __builtin_amdgcn_readfirstlane(sg.s.length);
+    sg.seq = __builtin_amdgcn_readfirstlane(sg.seq);
+    sg.head = __builtin_amdgcn_readfirstlane(sg.head);
+    sg.row0 = __builtin_amdgcn_readfirstlane(sg.row0);
+    sg.rows = __builtin_amdgcn_readfirstlane(sg.rows);
+    sg.keys = __builtin_amdgcn_readfirstlane(sg.keys);
+    sg.u0 = __builtin_amdgcn_readfirstlane(sg.u0);
+    sg.u1 = __builtin_amdgcn_readfirstlane(sg.u1);
+    sg.slot = __builtin_amdgcn_readfirstlane(sg.slot);
+    return sg;
+}
 
 /* tokens of the sequences of a launch, which begin at row `start` */
 __device__ __forceinline__ int prefix_tokens(const CachedParams & p, int start)
@@ -128,44 +147,47 @@ __device__ __forceinline__ int prefix_tokens(const CachedParams & p, int start)
     return min(max(min(p.c.starts[p.seq0 + p.seqs], p.c.tokens) - start, 0), most);
 }
 
-/* CACHED_TILES: the segment of workgroup `id`, tiles of TR rows, units of UK keys; false: it has none */
+/* CACHED_TILES: the segment of workgroup `id`, tiles of TR rows, units of UK keys; without rows where it has none */
 template <int TR, int UK>
-__device__ __forceinline__ bool tile_segment(const CachedParams & p, CachedScan & sh, int id, Segment & sg)
+__device__ __forceinline__ Segment tile_segment(const CachedParams & p, CachedScan & sh, int id)
 {
     /* the last tiles of a sequence see the most keys: first */
     const int perTile = p.c.kvHeads * p.groups;
-    int tile = p.tiles - 1 - id / perTile;
-    const int rest = id % perTile, piece = rest / p.c.kvHeads;
-    sg.head = rest - piece * p.c.kvHeads;
-    sg.slot = p.acc ? (tile * p.c.kvHeads + sg.head) * p.groups + piece : -1;
+    const int tile = p.tiles - 1 - id / perTile, rest = id % perTile, piece = rest / p.c.kvHeads;
+    int start, fresh, length, keys, seq = 0, row0 = tile * TR;
     if (p.prefix > 0) {
-        sg.s.start = cache_sequence(p.c, p.seq0).start;
-        sg.s.fresh = prefix_tokens(p, sg.s.start);
-        sg.s.length = p.prefix;
-        sg.seq = 0;
+        start = cache_sequence(p.c, p.seq0).start;
+        fresh = prefix_tokens(p, start);
+        length = keys = p.prefix;
     }
     else {
         const auto tiles = [&](int n) { return (long long)((cache_sequence(p.c, p.seq0 + n).fresh * p.per + TR - 1) / TR); };
         const SequenceScan scan = scan_sequences(p.seqs, sh, tiles);
-        long long before;
+        long long before = 0;
         const int i = find_sequence(scan, tile, before, sh, tiles);
-        if (i < 0)
-            return false;
-        tile -= (int)before;
-        sg.seq = p.seq0 + i;
-        sg.s = cache_sequence(p.c, sg.seq);
+        const CacheSequence s = cache_sequence(p.c, p.seq0 + max(i, 0));
+        start = s.start;
+        fresh = i < 0 ? 0 : s.fresh;
+        length = keys = s.length;
+        seq = p.seq0 + max(i, 0);
+        row0 -= (int)before * TR;
+        if (p.causal)
+            keys -= fresh - 1 - divided(max(min(row0 + TR, fresh * p.per) - 1, 0), p.perDiv);
     }
-    sg.rows = sg.s.fresh * p.per;
-    sg.row0 = tile * TR;
-    if (sg.row0 >= sg.rows)
-        return false;
-    int keys = sg.s.length;
-    if (p.causal && p.prefix == 0)
-        keys -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
     const int units = (max(keys - p.first, 0) + UK - 1) / UK, each = (units + p.groups - 1) / p.groups;
+    Segment sg;
+    sg.s.start = start;
+    sg.s.fresh = fresh;
+    sg.s.length = length;
+    sg.seq = seq;
+    sg.head = rest - piece * p.c.kvHeads;
+    sg.row0 = row0;
+    sg.rows = row0 < fresh * p.per ? fresh * p.per : 0;
+    sg.keys = keys;
     sg.u0 = min(each * piece, units);
     sg.u1 = min(sg.u0 + each, units);
-    return true;
+    sg.slot = p.acc ? (tile * p.c.kvHeads + sg.head) * p.groups + piece : -1;
+    return sg;
 }
 
 /* The sequences of this lane's rows (row0 + 16 q) in a launch over the shared prefix, whose rows are the tokens of all
@@ -204,39 +226,33 @@ __device__ __forceinline__ void row_sequences(const CachedParams & p, const Segm
         seq[q] = p.seq0 + max(count[q] - 1, 0);
 }
 
-/* How many positions this lane's rows (row0 + 16 q) see, the least and the most of the 16 lanes' rows. Rows that a
-   tile does not have see everything: they are computed with, never stored. */
+/* How many positions this lane's rows (row0 + 16 q) see, and the least of the 16 lanes' rows. Rows that a tile does not
+   have see everything: they are computed with, never stored. */
 template <int QR, int N>
-__device__ __forceinline__ void rows_seen(const CachedParams & p, const Segment & sg, int row0, int * from, int (&seen)[QR],
-                                          int & least, int & most)
+__device__ __forceinline__ int rows_seen(const CachedParams & p, const Segment & sg, int row0, int * from, int (&seen)[QR])
 {
+    int seq[QR] = {};
     if (p.prefix > 0 && p.c.starts)
-        row_sequences<QR, N>(p, sg, row0, from, seen);
-    least = 0x7fffffff;
-    most = 0;
+        row_sequences<QR, N>(p, sg, row0, from, seq);
+    int least = 0x7fffffff;
 #pragma unroll
     for (int q = 0; q < QR; q++) {
         const int row = row0 + 16 * q, t = divided(row, p.perDiv);
-        if (row >= sg.rows) {
-            seen[q] = 0x7fffffff;
-            continue;
+        int n = 0x7fffffff;
+        if (row < sg.rows) {
+            n = p.causal ? sg.s.length - sg.s.fresh + t + 1 : sg.s.length;
+            if (p.prefix > 0) {
+                const CacheSequence s = cache_sequence(p.c, p.c.starts ? seq[q] : p.seq0 + t / p.c.maxNew);
+                n = min(p.causal ? s.length - s.fresh + (sg.s.start + t - s.start) + 1 : s.length, p.prefix);
+            }
         }
-        if (p.prefix > 0) {
-            const CacheSequence s = cache_sequence(p.c, p.c.starts ? seen[q] : p.seq0 + t / p.c.maxNew);
-            seen[q] = min(p.causal ? s.length - s.fresh + (sg.s.start + t - s.start) + 1 : s.length, p.prefix);
-        }
-        else
-            seen[q] = p.causal ? sg.s.length - sg.s.fresh + t + 1 : sg.s.length;
-        least = min(least, seen[q]);
-        most = max(most, seen[q]);
+        seen[q] = n;
+        least = min(least, n);
     }
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) {
+    for (int d = 8; d >= 1; d >>= 1)
         least = min(least, __shfl_xor(least, d));
-        most = max(most, __shfl_xor(most, d));
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
+    return __builtin_amdgcn_readfirstlane(least);
 }
 
 /* The softmax of a row runs on raw scores s and the base-2 scale of p: 2^(s scale2 - shift). Scores are multiplied by |scale|
@@ -275,6 +291,12 @@ __device__ __forceinline__ long long lane_of(long long x, int source)
 {
     const int lo = __shfl((int)x, source), hi = __shfl((int)(x >> 32), source);
     return ((long long)hi << 32) | (unsigned)lo;
+}
+
+/* entry i of a row of the page table: a scalar base and a 32-bit offset (rows are below 4 GiB) */
+__device__ __forceinline__ int page_entry(const int * row, int i)
+{
+    return *(const __attribute__((address_space(1))) int *)((const __attribute__((address_space(1))) char *)row + (unsigned)i * 4u);
 }
 
 template <typename V>

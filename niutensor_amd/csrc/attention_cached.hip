@@ -91,8 +91,8 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     const int dh = c.dh;
 
     /* ---- this lane's query rows: positions each sees, fragments ---- */
-    int seen[QR], seenMin, seenMax;
-    rows_seen<QR, 4096>(p, sg, sg.row0 + m, reinterpret_cast<int *>(&sh.acc[0][0][0]), seen, seenMin, seenMax);
+    int seen[QR];
+    const int seenMin = rows_seen<QR, 4096>(p, sg, sg.row0 + m, reinterpret_cast<int *>(&sh.acc[0][0][0]), seen);
     typename U::KPiece qf[QR][U::NT];
 #pragma unroll
     for (int q = 0; q < QR; q++) {
@@ -117,7 +117,7 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     const int myKey = lane & (U::UK - 1);
     auto page_of = [&](int u) {
         const int key = p.first + u * U::UK + myKey;
-        return u < sg.u1 && key < seenMax ? table[divided(key, c.pageSize)] : -1;
+        return u < sg.u1 && key < sg.keys ? page_entry(table, divided(key, c.pageSize)) : -1;
     };
     /* byte offsets of a lane's columns in a row. Columns past dh read the row's first: a key's meet zeros of q, a value's
        end in columns of the result that are not stored */
@@ -318,34 +318,48 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     }
 }
 
-/* CACHED_PIECES: the segment of workgroup `id`; false: it has none */
+/* CACHED_WHOLE, CACHED_PIECES: the segment of workgroup `id`; without rows where it has none */
 template <int UK>
-__device__ __forceinline__ bool piece_segment(const CachedParams & p, CachedScan & sh, int id, Segment & sg)
+__device__ __forceinline__ Segment pair_segment(const CachedParams & p, CachedScan & sh, int id)
 {
-    const PiecePlan f = piece_plan<UK>(p, sh);
-    long long before;
-    const int i = find_sequence(f.scan, id, before, sh, [&](int n) { return pieces_of<UK>(p, n, f.most); });
-    if (i < 0)
-        return false;
+    int i, head, u0 = 0, u1 = 0x7fffffff, slot;
+    if (p.mode == CACHED_PIECES) {
+        const PiecePlan f = piece_plan<UK>(p, sh);
+        long long before = 0;
+        const int found = find_sequence(f.scan, id, before, sh, [&](int n) { return pieces_of<UK>(p, n, f.most); });
+        i = max(found, 0);
+        const int units = found < 0 ? 0 : units_of<UK>(p, cache_sequence(p.c, p.seq0 + i));
+        const int pieces = (int)(((unsigned)units + f.most - 1) / (unsigned)f.most);
+        /* the key heads of a piece side by side: their rows may be neighbours in memory */
+        const int in = id - (int)before, piece = in / p.c.kvHeads;
+        head = in - piece * p.c.kvHeads;
+        u0 = piece * f.most;
+        u1 = found < 0 ? -1 : u0 + f.most;
+        /* slots of cut pairs are numbered through; behind a prefix the others have one each after those */
+        const int pair = i * p.c.kvHeads + head;
+        const int slot0 = pieces > 1 ? (int)(before >> 32) + head * pieces : (p.first > 0 ? 2 * p.groups + pair : -1);
+        slot = slot0 < 0 ? -1 : slot0 + piece;
+        if (found >= 0 && piece == 0 && threadIdx.x == 0) {
+            p.slots[2 * pair] = slot0;
+            p.slots[2 * pair + 1] = slot0 < 0 ? 0 : pieces;
+        }
+    }
+    else {
+        i = id / p.c.kvHeads;
+        head = id - i * p.c.kvHeads;
+        slot = p.acc ? id : -1;
+    }
+    Segment sg;
     sg.seq = p.seq0 + i;
     sg.s = cache_sequence(p.c, sg.seq);
-    const int units = units_of<UK>(p, sg.s), pieces = (int)(((unsigned)units + f.most - 1) / (unsigned)f.most);
-    /* the key heads of a piece side by side: their rows may be neighbours in memory */
-    const int in = id - (int)before, piece = in / p.c.kvHeads;
-    sg.head = in - piece * p.c.kvHeads;
+    sg.head = head;
     sg.row0 = 0;
-    sg.rows = sg.s.fresh * p.per;
-    sg.u0 = piece * f.most;
-    sg.u1 = min(sg.u0 + f.most, units);
-    /* slots of cut pairs are numbered through; behind a prefix the others have one each after those */
-    const int pair = i * p.c.kvHeads + sg.head;
-    const int slot0 = pieces > 1 ? (int)(before >> 32) + sg.head * pieces : (p.first > 0 ? 2 * p.groups + pair : -1);
-    sg.slot = slot0 < 0 ? -1 : slot0 + piece;
-    if (piece == 0 && threadIdx.x == 0) {
-        p.slots[2 * pair] = slot0;
-        p.slots[2 * pair + 1] = slot0 < 0 ? 0 : pieces;
-    }
-    return true;
+    sg.rows = u1 < 0 ? 0 : sg.s.fresh * p.per;
+    sg.keys = sg.s.length;
+    sg.u0 = u0;
+    sg.u1 = min(u1, (max(sg.s.length - p.first, 0) + UK - 1) / UK);
+    sg.slot = slot;
+    return sg;
 }
 
 template <typename T, int DHM, int QR>
@@ -355,29 +369,9 @@ attention_cached_kernel(const CachedParams p)
     constexpr int UK = Unit<T, DHM>::UK, TR = 16 * QR;
     __shared__ CachedShared sh;
     const int id = (int)blockIdx.x;
-    Segment sg;
-    if (p.mode == CACHED_TILES) {
-        if (!tile_segment<TR, UK>(p, sh.scan, id, sg))
-            return;
-    }
-    else if (p.mode == CACHED_PIECES) {
-        if (!piece_segment<UK>(p, sh.scan, id, sg))
-            return;
-    }
-    else {
-        const int i = id / p.c.kvHeads;
-        sg.head = id - i * p.c.kvHeads;
-        sg.seq = p.seq0 + i;
-        sg.s = cache_sequence(p.c, sg.seq);
-        sg.row0 = 0;
-        sg.rows = sg.s.fresh * p.per;
-        sg.u0 = 0;
-        sg.u1 = (max(sg.s.length - p.first, 0) + UK - 1) / UK;
-        sg.slot = p.acc ? id : -1;
-        if (sg.rows == 0)
-            return;
-    }
-    attend<T, DHM, QR>(p, sg, sh);
+    const Segment sg = uniform(p.mode == CACHED_TILES ? tile_segment<TR, UK>(p, sh.scan, id) : pair_segment<UK>(p, sh.scan, id));
+    if (sg.rows > 0)
+        attend<T, DHM, QR>(p, sg, sh);
 }
 
 template <typename T, int DHM>

@@ -41,21 +41,18 @@ attention_cached_tiles_kernel(const CachedParams p)
     const int m = lane & 15, g = lane >> 4;
     const int dh = c.dh;
 
-    Segment sg;
-    if (!tile_segment<TR, KB>(p, scan, (int)blockIdx.x, sg))
+    const Segment sg = uniform(tile_segment<TR, KB>(p, scan, (int)blockIdx.x));
+    if (sg.rows == 0)
         return;
     const int row0 = sg.row0 + wave * (16 * QR) + m;
-    int seen[QR], seenMin, seenMax;
-    rows_seen<QR, KB * PITCH / 4>(p, sg, row0, reinterpret_cast<int *>(Ks), seen, seenMin, seenMax);
+    int seen[QR];
+    const int seenMin = rows_seen<QR, KB * PITCH / 4>(p, sg, row0, reinterpret_cast<int *>(Ks), seen);
 
     /* ---- where the keys of a block stand: lane l looks after key l ---- */
     const int * table = c.table + (long long)sg.seq * c.tablePages;
-    int keyEnd = sg.s.length;                /* the keys that any row of the tile sees */
-    if (p.causal && p.prefix == 0)
-        keyEnd -= sg.s.fresh - 1 - divided(min(sg.row0 + TR, sg.rows) - 1, p.perDiv);
     auto page_of = [&](int u) {
         const int key = p.first + u * KB + lane;
-        return u < sg.u1 && key < keyEnd ? table[divided(key, c.pageSize)] : -1;
+        return u < sg.u1 && key < sg.keys ? page_entry(table, divided(key, c.pageSize)) : -1;
     };
     const int sr0 = tid / TPR, sc = (tid % TPR) * 8;
     const int sLds = sr0 * PITCH + sc * 2;

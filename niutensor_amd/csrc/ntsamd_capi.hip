@@ -1005,7 +1005,7 @@ int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, Ca
         return fail(NTSAMD_ERR_ARGUMENT, "sequences of %d positions, but %d pages of %d in a row of the page table",
                     batch->maxLength, batch->tablePages, cache->pageSize);
     const long long maxLength = batch->maxLength > 0 ? batch->maxLength : positions;
-    if (maxLength > 0x7fff0000LL)
+    if (maxLength > 0x7fff0000LL || batch->tablePages > 0x3fffffff)
         return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
     if (!batch->starts && (long long)batch->sequences * batch->maxNew > batch->tokens)
         return fail(NTSAMD_ERR_ARGUMENT, "%d sequences of %d new tokens, but %d rows", batch->sequences, batch->maxNew, batch->tokens);
