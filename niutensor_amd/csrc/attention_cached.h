@@ -309,6 +309,10 @@ int launch_attention_cached(const CachedParams & p, bool half, int qr, int block
 /* CACHED_TILES of half tensors, tiles of 64 qr rows (qr 1 or 2) */
 int launch_attention_cached_tiles(const CachedParams & p, int qr, int blocks, hipStream_t stream);
 constexpr int CACHED_TILE_KEYS = 64;
+/* both launches of a shared prefix in one: `pre` over it in tiles of `tile` rows (64 or 128 half, 16 or 32 float), `own` over each
+   sequence's own keys, 16 qr rows */
+int launch_attention_prefix(const CachedParams & pre, const CachedParams & own, bool half, int tile, int qr, int preBlocks,
+                            int ownBlocks, hipStream_t stream);
 
 /* the partial results of a launch (p.acc, p.stat), and of the launch over the shared prefix before it, to p.out */
 struct JoinParams {

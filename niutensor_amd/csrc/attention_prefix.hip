@@ -1,0 +1,83 @@
+/*
+ * Attention behind a shared prefix (ntsamd_attention_prefix): in one launch, workgroups that multiply the queries of all
+ * sequences with the prefix, as tiles of one matrix, and workgroups that take each sequence's own keys. The first
+ * wait on matrix instructions, the second on memory; taken in turn, eight of one kind and eight of the other (a workgroup
+ * for each XCD), a CU has both. attention_join_kernel puts their partial results together.
+ * 64 sequences of 8193 to 8704 positions behind a prefix of 8192, 8 key heads of 128, four query heads to each, half: 28 us
+ * and 23 us one after the other.
+ */
+#include "attention_cached_rows.h"
+#include "attention_cached_tiles.h"
+
+namespace ntsamd {
+
+namespace {
+
+/* TILE: rows of a tile of the prefix (16 and 32 float, 64 and 128 half); QR: blocks of 16 rows of a sequence's own */
+template <typename T, int DHM, int TILE, int QR>
+__global__ void __launch_bounds__(256, DHM == 128 && (QR == 2 || TILE == 32) ? 1 : 2)
+attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preBlocks, int ownBlocks)
+{
+    __shared__ union Shared {
+        CachedShared rows;
+        CachedTilesShared<DHM> tiles;
+        __device__ Shared() {}
+    } sh;
+    const int id = (int)blockIdx.x, both = 2 * (min(preBlocks, ownBlocks) & ~7);
+    bool first;
+    int at;
+    if (id < both) {
+        first = ((id >> 3) & 1) == 0;
+        at = (id >> 4) * 8 + (id & 7);
+    }
+    else {
+        at = id - both / 2;
+        first = at < preBlocks;
+        if (!first)
+            at -= preBlocks - both / 2;
+    }
+    if (first) {
+        if constexpr (TILE > 32)
+            attend_tile<DHM, TILE / 64>(pre, at, sh.tiles);
+        else
+            attend_tile_rows<T, DHM, TILE / 16>(pre, at, sh.rows);
+    }
+    else
+        attend_pair<T, DHM, QR>(own, at, sh.rows);
+}
+
+template <typename T, int DHM, int TILE>
+int launch_tile(const CachedParams & pre, const CachedParams & own, int qr, int preBlocks, int ownBlocks, hipStream_t stream)
+{
+    const dim3 grid((unsigned)(preBlocks + ownBlocks)), block(256);
+    if (qr == 1)
+        hipLaunchKernelGGL((attention_prefix_kernel<T, DHM, TILE, 1>), grid, block, 0, stream, pre, own, preBlocks, ownBlocks);
+    else
+        hipLaunchKernelGGL((attention_prefix_kernel<T, DHM, TILE, 2>), grid, block, 0, stream, pre, own, preBlocks, ownBlocks);
+    return (int)hipGetLastError();
+}
+
+template <int DHM>
+int launch_dhm(const CachedParams & pre, const CachedParams & own, bool half, int tile, int qr, int preBlocks, int ownBlocks,
+               hipStream_t stream)
+{
+    if (half)
+        return tile <= 64 ? launch_tile<half_t, DHM, 64>(pre, own, qr, preBlocks, ownBlocks, stream)
+                          : launch_tile<half_t, DHM, 128>(pre, own, qr, preBlocks, ownBlocks, stream);
+    return tile <= 16 ? launch_tile<float, DHM, 16>(pre, own, qr, preBlocks, ownBlocks, stream)
+                      : launch_tile<float, DHM, 32>(pre, own, qr, preBlocks, ownBlocks, stream);
+}
+
+}  // namespace
+
+int launch_attention_prefix(const CachedParams & pre, const CachedParams & own, bool half, int tile, int qr, int preBlocks,
+                            int ownBlocks, hipStream_t stream)
+{
+    if (pre.c.dh <= 32)
+        return launch_dhm<32>(pre, own, half, tile, qr, preBlocks, ownBlocks, stream);
+    if (pre.c.dh <= 64)
+        return launch_dhm<64>(pre, own, half, tile, qr, preBlocks, ownBlocks, stream);
+    return launch_dhm<128>(pre, own, half, tile, qr, preBlocks, ownBlocks, stream);
+}
+
+}  // namespace ntsamd

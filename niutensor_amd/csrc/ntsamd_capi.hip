@@ -1052,7 +1052,6 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     const auto tile_kernel = [](int tile) { return tile > 32 ? "attention_cached_tiles_kernel" : "attention_cached_kernel"; };
     WorkHold work;
     int rc = 0;
-    char text[160] = "";
     p.seq0 = 0;
     p.seqs = n;
     p.first = 0;
@@ -1108,75 +1107,65 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         p.rows = (int)rows;
         const long long room = (long long)SPLIT_WORK_BYTES / slotRow;       /* partial rows that fit */
         const bool shared = prefix >= 4 * unit && n > 1 && mayHold && 512LL * kv <= room;
-        const long long own = p.c.maxLength - (shared ? prefix : 0);
-        bool flat = mayHold && units(own) > 8;
-        if (shared || flat) {
+        if (shared || (mayHold && units(p.c.maxLength) > 8))
             work.take_stream(devID, stream);
-            if (work.mem == NULL)
-                flat = false;
-        }
         const bool withPrefix = shared && work.mem != NULL;
         if (!withPrefix)
-            flat = mayHold && work.mem != NULL && units(p.c.maxLength) > 8;
+            prefix = 0;
+        const long long own = p.c.maxLength - prefix;
+        const bool cut = work.mem != NULL && units(own) > 8;
         /* with a prefix every row has a partial result of its own keys beside those of the prefix's pieces */
         int step = n;
         if (withPrefix) {
             const long long most = room / 4 / (rows * kv);
             step = most < n ? (most > 1 ? (int)most : 1) : n;
         }
-        if (!withPrefix)
-            prefix = 0;
         if ((long long)step * kv * rows > 0x7fffffffLL / 64)
             return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
         for (int seq0 = 0; seq0 < n && rc == 0; seq0 += step) {
-            CachedParams o = p;
+            CachedParams o = p, pre;                    /* each sequence's own keys; the prefix */
             o.seq0 = seq0;
             o.seqs = n - seq0 < step ? n - seq0 : step;
+            o.first = prefix;
             const long long pairs = (long long)o.seqs * kv;
-            JoinParams j;
-            memset(&j, 0, sizeof(j));
-            long long used = 0;
+            long long used = 0, preBlocks = 0;
             if (withPrefix) {
-                CachedParams s = o;
                 const long long all = o.seqs * rows;
-                s.mode = CACHED_TILES;
-                s.prefix = prefix;
-                s.rows = tile_rows(all);
-                s.tiles = (int)((all + s.rows - 1) / s.rows);
-                const long long slots = (long long)s.tiles * kv;
-                long long pieces = (2 * cus + slots - 1) / slots;
-                const int keys = s.rows > 32 ? CACHED_TILE_KEYS : 4 * unit;
-                const long long most = (prefix + keys - 1) / keys, fit = room / 2 / (slots * s.rows);
+                pre = o;
+                pre.mode = CACHED_TILES;
+                pre.first = 0;
+                pre.prefix = prefix;
+                pre.rows = half ? (all <= 64 ? 64 : 128) : (all <= 16 ? 16 : 32);
+                pre.tiles = (int)((all + pre.rows - 1) / pre.rows);
+                /* one workgroup to a CU beside those of the sequences' own keys, two if there are few of these; at least a
+                   round of keys each */
+                const long long slots = (long long)pre.tiles * kv, keys = half ? CACHED_TILE_KEYS : 4 * unit;
+                long long pieces = ((pairs < cus / 2 ? 2 : 1) * cus + slots - 1) / slots;
+                const long long most = (prefix + keys - 1) / keys, fit = room / 2 / (slots * pre.rows);
                 pieces = pieces < most ? pieces : most;
                 pieces = pieces < fit ? pieces : fit;
-                if (pieces < 1)
-                    pieces = 1;
-                s.groups = (int)pieces;
-                s.acc = work.mem;
-                s.stat = s.acc + slots * pieces * s.rows * dh;
-                used = slots * pieces * s.rows;
-                j.preAcc = s.acc;
-                j.preStat = s.stat;
-                j.prePieces = s.groups;
-                j.preRows = s.rows;
-                snprintf(text, sizeof(text), "%s prefix tiles=%dx%d pieces=%lld+", tile_kernel(s.rows), s.tiles, s.rows, pieces);
-                if (!g_planOnly)
-                    rc = launch(s, s.rows, slots * pieces);
+                pre.groups = (int)(pieces < 1 ? 1 : pieces);
+                preBlocks = slots * pre.groups;
+                used = preBlocks * pre.rows;
+                pre.acc = work.mem;
+                pre.stat = pre.acc + used * dh;
             }
-            o.first = prefix;
             long long blocks = pairs;
             o.mode = CACHED_WHOLE;
-            if (flat) {
+            if (cut) {
                 /* what is left holds 2 `groups` slots, one more for each pair behind a prefix, and two numbers for each pair */
                 const long long left = room - used - (withPrefix ? pairs * rows : 0) - (pairs * 8 + slotRow - 1) / slotRow;
-                long long groups = tuning().groupM.load() > 0 ? tuning().groupM.load() : 4 * cus;
+                /* Pieces aimed at: two to a CU, which all run at once (two workgroups fit a CU with heads of more than 64
+                   columns, three or four with fewer); a pair's last piece may be short, so wide heads with many pairs do
+                   better in two rounds of smaller pieces. 64 sequences to 8191 positions x 8 heads of 128: 219 us with
+                   two to a CU, 206 with four; one sequence of 131072: 101 and 106; 124 to 2890 x 4 of 32: 31.5 and 34. */
+                long long groups = (dh > 64 && pairs >= cus / 2 ? 4 : 2) * cus;
                 groups = groups < left / (2 * rows) ? groups : left / (2 * rows);
                 if (groups >= cus / 2) {
                     o.mode = CACHED_PIECES;
                     o.groups = (int)groups;
-                    blocks = groups + pairs;
                     const long long most = pairs * ((units(own) + 3) / 4);
-                    blocks = blocks < most ? blocks : most;
+                    blocks = groups + pairs < most ? groups + pairs : most;
                 }
             }
             if (withPrefix || o.mode == CACHED_PIECES) {
@@ -1185,14 +1174,25 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 o.stat = o.acc + slots * rows * dh;
                 o.slots = reinterpret_cast<int *>(o.stat + 2 * slots * rows);
             }
-            snprintf(g_plan, sizeof(g_plan), "%sattention_cached_kernel rows=%d %s=%lld%s", text, tile,
-                     o.mode == CACHED_PIECES ? "pieces" : "whole", blocks, o.acc ? "+attention_join_kernel" : "");
+            char text[96] = "attention_cached_kernel";
+            if (withPrefix)
+                snprintf(text, sizeof(text), "attention_prefix_kernel tiles=%dx%d pieces=%d", pre.tiles, pre.rows, pre.groups);
+            snprintf(g_plan, sizeof(g_plan), "%s rows=%d %s=%lld%s", text, tile, o.mode == CACHED_PIECES ? "pieces" : "whole", blocks,
+                     o.acc ? "+attention_join_kernel" : "");
             if (g_planOnly)
                 return NTSAMD_OK;
-            if (rc == 0)
-                rc = launch(o, tile, blocks);
+            rc = withPrefix ? launch_attention_prefix(pre, o, half, pre.rows, tile / 16, (int)preBlocks, (int)blocks, stream)
+                            : launch(o, tile, blocks);
             if (rc == 0 && o.acc) {
+                JoinParams j;
+                memset(&j, 0, sizeof(j));
                 j.p = o;
+                if (withPrefix) {
+                    j.preAcc = pre.acc;
+                    j.preStat = pre.stat;
+                    j.prePieces = pre.groups;
+                    j.preRows = pre.rows;
+                }
                 rc = launch_attention_join(j, half, (int)(pairs * rows), stream);
             }
         }
