@@ -6,39 +6,57 @@
  * Bound by the matrix instructions and what feeds them, so keys and values go through LDS once for all rows of a
  * workgroup, on the plan of attention_f16.hip: 64 QR rows (tokens x the query heads that share a key head) of a tile, 16 QR
  * per wave; blocks of 64 keys; both products transposed, so that probabilities pass from accumulator to operand inside
- * a lane; values read back by transposing LDS reads. What is different is where the keys stand: lane l of every wave looks
- * up the page of key l of a block, one block ahead, and hands its address to the lanes that fetch the row. Rows of a
+ * a lane; values read back by transposing LDS reads. What is different: lane l of every wave looks
+ * up the page of key l of a block, one block ahead, and hands its address to the lanes that fetch the row; rows go from memory
+ * to LDS without registers in between, a block ahead, two stages, one barrier a block; the sums of the probabilities are one
+ * more product, with a row of ones (of the rounded probabilities then, as the results are), since the vector ALU's exponentials and
+ * conversions are what a wave spends most of its time on. Rows of a
  * tile see different numbers of keys; only the blocks in which some row's last key falls, or which have an absent page, take the
  * comparisons. Fetches of keys that a tile does not have read a row of zeros.
  */
 #pragma once
 #include "gemm_common.h"
-#include "gemm_f16.h"       /* half_t, lds_read_tr16 */
+#include "gemm_f16_direct.h"        /* half_t, lds_read_tr16, wait_vmcnt, wait_lgkmcnt0 */
 #include "attention.h"
 #include "attention_cached.h"
 
 namespace ntsamd {
 
+/* Two stages of a block of keys and values. Rows are 2 DHM bytes, without padding (they are written 16 bytes a lane, one
+   lane after the other); which 16-byte piece of a row stands where is swizzled by the row instead, so that 16 rows read
+   at one column, and the pairs of pieces that a transposing read takes of 8 rows, spread over all banks. */
 template <int DHM> struct CachedTilesShared {
-    static constexpr int PITCH = DHM * 2 + 16;      /* bytes per LDS row: 16 mod 128, so 16-byte reads of consecutive rows
-                                                       walk through the banks */
-    __attribute__((aligned(16))) char k[CACHED_TILE_KEYS * PITCH];
-    __attribute__((aligned(16))) char v[CACHED_TILE_KEYS * PITCH];
+    static constexpr int PIECES = DHM / 8, BLOCK = CACHED_TILE_KEYS * DHM * 2;
+    __attribute__((aligned(1024))) char k[2][BLOCK];
+    __attribute__((aligned(1024))) char v[2][BLOCK];
     CachedScan scan;
+    static __device__ __forceinline__ int swizzle(int row)
+    {
+        const int k = (row & 15) * PIECES / 16;         /* rows that share the 256 bytes of a round of banks take the same */
+        return ((k & (PIECES / 2 - 1)) << 1) | (k / (PIECES / 2));
+    }
 };
+
+/* global memory -> LDS, 16 bytes per lane: lane l's data lands at lds + 16 l (the same for the whole wave). Counted by vmcnt, which
+   the caller waits for: the compiler does not see a load */
+__device__ __forceinline__ void lds_from_global16(unsigned lds, long long address)
+{
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds), "v"(address)
+                 : "memory");
+}
 
 /* workgroup `id` of a CACHED_TILES launch over half tensors, tiles of 64 QR rows */
 template <int DHM, int QR>
 __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, CachedTilesShared<DHM> & sh)
 {
+    typedef CachedTilesShared<DHM> Shared;
     constexpr int KB = CACHED_TILE_KEYS, TR = 64 * QR;
-    constexpr int PITCH = CachedTilesShared<DHM>::PITCH;
     constexpr int NT = DHM / 32, ND = DHM / 16, NJ = KB / 16;
-    constexpr int TPR = DHM / 8;             /* threads per row when staging */
-    constexpr int RSTEP = 256 / TPR, LOADS = KB / RSTEP;
+    constexpr int PIECES = Shared::PIECES, ROWS = 64 / PIECES;          /* rows of a block that a wave fetches at a time */
+    constexpr int LOADS = KB / (4 * ROWS);
 
-    char * const Ks = sh.k;
-    char * const Vs = sh.v;
     const CacheParams & c = p.c;
     const int tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -50,7 +68,7 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
         return;
     const int row0 = sg.row0 + wave * (16 * QR) + m;
     int seen[QR];
-    const int seenMin = rows_seen<QR, KB * PITCH / 4>(p, sg, row0, reinterpret_cast<int *>(Ks), seen);
+    const int seenMin = rows_seen<QR, Shared::BLOCK / 4>(p, sg, row0, reinterpret_cast<int *>(sh.k[0]), seen);
 
     /* ---- where the keys of a block stand: lane l looks after key l ---- */
     const int * table = c.table + (long long)sg.seq * c.tablePages;
@@ -58,29 +76,32 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
         const int key = p.first + u * KB + lane;
         return u < sg.u1 && key < sg.keys ? page_entry(table, divided(key, c.pageSize)) : -1;
     };
-    const int sr0 = tid / TPR, sc = (tid % TPR) * 8;
-    const int sLds = sr0 * PITCH + sc * 2;
-    f16x8 kreg[LOADS], vreg[LOADS];
+    /* the rows that this lane fetches a piece of: row `fetch` + ROWS s of the block */
+    const int fetch = wave * (LOADS * ROWS) + lane / PIECES;
+    int col[LOADS];                          /* columns past dh: the row's first, which meet zeros of q or are not stored */
+#pragma unroll
+    for (int s = 0; s < LOADS; s++) {
+        const int at = 16 * ((lane % PIECES) ^ Shared::swizzle(fetch + ROWS * s));
+        col[s] = at < 2 * dh ? at : 0;
+    }
+    const unsigned kLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.k[0]) + wave * (LOADS * 1024);
+    const unsigned vLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.v[0]) + wave * (LOADS * 1024);
     unsigned long long there = 0;            /* which keys of the block being fetched exist */
-    long long vRow = 0;
-    const int col = sc < dh ? 2 * sc : 0;    /* columns past dh: the row's first, which meet zeros of q or are not stored */
-    auto load_k = [&](int u, int page) {
+    auto fetch_block = [&](int u, int page) {
         const KeyPlace at = key_place<half_t>(c, sg.head, p.first + u * KB + lane, page);
-        vRow = at.v;
+        const unsigned stage = ((u - sg.u0) & 1) * Shared::BLOCK;
         there = __ballot(at.there);
 #pragma unroll
         for (int s = 0; s < LOADS; s++)
-            kreg[s] = load_global<f16x8>(lane_of(at.k, sr0 + s * RSTEP) + col);
-    };
-    auto load_v = [&]() {
+            lds_from_global16(kLds + stage + s * 1024, lane_of(at.k, fetch + ROWS * s) + col[s]);
 #pragma unroll
         for (int s = 0; s < LOADS; s++)
-            vreg[s] = load_global<f16x8>(lane_of(vRow, sr0 + s * RSTEP) + col);
+            lds_from_global16(vLds + stage + s * 1024, lane_of(at.v, fetch + ROWS * s) + col[s]);
     };
-    int page = page_of(sg.u0);
-    load_k(sg.u0, page);
-    load_v();
-    page = page_of(sg.u0 + 1);
+    /* rows_seen may have had numbers in the first stage: every lane is past its last read of them */
+    if (sg.u0 < sg.u1)
+        fetch_block(sg.u0, page_of(sg.u0));
+    int page = page_of(sg.u0 + 1);
 
     /* ---- Q fragments ---- */
     f16x8 qf[QR][NT];
@@ -101,28 +122,44 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
         }
     }
 
-    f32x4 accO[QR][ND];
-    float rowMax[QR], rowSum[QR];
+    f32x4 accO[QR][ND], accL[QR];            /* accL: the sum of the row's probabilities, in every register */
+    float rowMax[QR];
 #pragma unroll
     for (int q = 0; q < QR; q++) {
 #pragma unroll
         for (int d = 0; d < ND; d++)
             accO[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        accL[q] = f32x4{0.f, 0.f, 0.f, 0.f};
         rowMax[q] = -INFINITY;
-        rowSum[q] = 0.f;
     }
     const float scale2 = score_scale(p);
-    /* where this lane points for the transposing reads: row 4 g + (m / 4) of a 16-key block, columns 4 (m % 4) .. + 3 */
-    const int trOff = (4 * g + (m >> 2)) * PITCH + (m & 3) * 8;
+    const half_t one = (half_t)1.f;
+    const f16x8 ones = {one, one, one, one, one, one, one, one};
+    /* where this lane reads keys (row m of a 16-key block, piece 4 t + g) and points for the transposing reads of values (row
+       4 g + m / 4, columns 16 d + 4 (m % 4) .. + 3) */
+    int kAt[NT], vAt[ND];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+        kAt[t] = m * (2 * DHM) + 16 * ((4 * t + g) ^ Shared::swizzle(m));
+    const int trRow = 4 * g + (m >> 2);
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+        vAt[d] = trRow * (2 * DHM) + 16 * ((2 * d + ((m & 3) >> 1)) ^ Shared::swizzle(trRow)) + 8 * (m & 1);
 
     for (int u = sg.u0; u < sg.u1; u++) {
         const int key0 = p.first + u * KB;
         const unsigned long long exist = there;
-#pragma unroll
-        for (int s = 0; s < LOADS; s++)
-            *reinterpret_cast<f16x8 *>(&Ks[sLds + s * RSTEP * PITCH]) = kreg[s];
-        __syncthreads();
-        load_k(u + 1, page);                 /* past the end: rows of zeros */
+        const char * const Ks = sh.k[(u - sg.u0) & 1];
+        const char * const Vs = sh.v[(u - sg.u0) & 1];
+        /* this block has landed, for every wave, and nobody reads the other stage any more: it is filled while this one is
+           worked on */
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<0>();
+        wait_lgkmcnt0();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (u + 1 < sg.u1)
+            fetch_block(u + 1, page);
         page = page_of(u + 2);
 
         /* ---- S^T = K Q^T ---- */
@@ -136,7 +173,7 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                const f16x8 kf = *reinterpret_cast<const f16x8 *>(&Ks[(16 * j + m) * PITCH + 64 * t + 16 * g]);
+                const f16x8 kf = *reinterpret_cast<const f16x8 *>(&Ks[kAt[t] + 16 * j * (2 * DHM)]);
 #pragma unroll
                 for (int q = 0; q < QR; q++)
                     accS[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[q][t], accS[q][j], 0, 0, 0);
@@ -173,7 +210,7 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
             for (int q = 0; q < QR; q++) {
                 const float newMax = fmaxf(rowMax[q], top[q]);
                 const float corr = __builtin_amdgcn_exp2f(rowMax[q] - (newMax == -INFINITY ? 0.f : newMax));
-                rowSum[q] *= corr;
+                accL[q] *= corr;
                 rowMax[q] = newMax;
 #pragma unroll
                 for (int d = 0; d < ND; d++)
@@ -186,27 +223,23 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(accS[q][j][r], scale2, -shift));
-                    rowSum[q] += e;                      /* this lane's keys only: the four lanes of a row meet at the end */
-                    pf[q][j][r] = (half_t)e;
-                }
+                for (int r = 0; r < 4; r++)
+                    pf[q][j][r] = (half_t)__builtin_amdgcn_exp2f(fmaf(accS[q][j][r], scale2, -shift));
         }
-
-#pragma unroll
-        for (int s = 0; s < LOADS; s++)
-            *reinterpret_cast<f16x8 *>(&Vs[sLds + s * RSTEP * PITCH]) = vreg[s];
-        __syncthreads();
-        load_v();
 
         /* ---- O^T += V^T P^T, 32 keys per MFMA: its k index 8 g + e stands for key 4 g + e of the first 16-key block of a
            pair for e < 4 and for key 4 g + e - 4 of the second for e >= 4 ---- */
 #pragma unroll
-        for (int j = 0; j < NJ; j += 2)
+        for (int j = 0; j < NJ; j += 2) {
+#pragma unroll
+            for (int q = 0; q < QR; q++) {
+                const f16x8 pp = __builtin_shufflevector(pf[q][j], pf[q][j + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                accL[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pp, accL[q], 0, 0, 0);
+            }
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                const f16x4 lo = lds_read_tr16(reinterpret_cast<const half_t *>(&Vs[16 * j * PITCH + trOff + 32 * d]));
-                const f16x4 hi = lds_read_tr16(reinterpret_cast<const half_t *>(&Vs[16 * (j + 1) * PITCH + trOff + 32 * d]));
+                const f16x4 lo = lds_read_tr16(reinterpret_cast<const half_t *>(&Vs[vAt[d] + 16 * j * (2 * DHM)]));
+                const f16x4 hi = lds_read_tr16(reinterpret_cast<const half_t *>(&Vs[vAt[d] + 16 * (j + 1) * (2 * DHM)]));
                 const f16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int q = 0; q < QR; q++) {
@@ -214,12 +247,13 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
                     accO[q][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp, accO[q][d], 0, 0, 0);
                 }
             }
+        }
     }
 
     /* ---- register r of block d is column 16 d + 4 g + r of the lane's row ---- */
 #pragma unroll
     for (int q = 0; q < QR; q++) {
-        const float total = lane_groups_sum(rowSum[q]);
+        const float total = accL[q][0];
         const int row = row0 + 16 * q;
         if (row >= sg.rows)
             continue;
