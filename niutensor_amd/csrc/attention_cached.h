@@ -321,6 +321,6 @@ struct JoinParams {
     const float * preStat;
     int prePieces, preRows;             /* pieces of its keys, rows of its tiles */
 };
-int launch_attention_join(const JoinParams & j, bool half, int blocks, hipStream_t stream);
+int launch_attention_join(const JoinParams & j, bool half, long long rows, hipStream_t stream);
 
 }  // namespace ntsamd

@@ -8,7 +8,7 @@ namespace ntsamd {
 namespace {
 
 template <typename T, int DHM, int QR>
-__global__ void __launch_bounds__(256, QR == 2 && DHM == 128 ? 1 : 2)
+__global__ void __launch_bounds__(256, 2)
 attention_cached_kernel(const CachedParams p)
 {
     __shared__ CachedShared sh;

@@ -2,8 +2,8 @@
  * The partial results of the cached attention (attention_cached.hip) joined: a row's pieces i, each an unnormalised row
  * a_i with the maximum m_i and the sum l_i of its softmax (base 2), give
  *   out = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i,   M = max_i m_i.
- * One workgroup per row: lanes of 4 columns, eight groups of them, which take the pieces in turn, in the order of the
- * keys, and meet in LDS in a fixed order, so results are the same bits on every run.
+ * A lane takes 4 columns of the pieces of a row, in the order of the keys; where a row may have many pieces eight groups of
+ * lanes take them in turn and meet in LDS, in a fixed order, so results are the same bits on every run.
  */
 #include "gemm_common.h"
 #include "gemm_f16.h"       /* half_t */
@@ -13,19 +13,24 @@ namespace ntsamd {
 
 namespace {
 
-template <typename T>
+/* TILES: the rows of tiles of one launch, every one in the same few pieces: eight rows to a workgroup, a group of lanes each.
+   Otherwise a row to a workgroup. */
+template <typename T, bool TILES>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(const JoinParams j)
 {
     __shared__ CachedScan sh;
-    __shared__ float partAcc[8][128], partStat[8][2];
+    __shared__ float partAcc[TILES ? 1 : 8][128], partStat[8][2];
     const CachedParams & p = j.p;
-    const int id = (int)blockIdx.x, kv = p.c.kvHeads;
-    const int unit = id / p.rows, row = id - unit * p.rows;     /* a pair or a tile, and a row of it */
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, col = 4 * lane;
+    const int kv = p.c.kvHeads, dh = p.c.dh;
+    /* tiles have multiples of 8 rows: those of a workgroup are of one tile */
+    const int first = (int)blockIdx.x * (TILES ? 8 : 1), id = TILES ? first + group : first;
+    const int unit = first / p.rows, row = id - unit * p.rows;  /* a pair or a tile, and a row of it */
     int head, inSeq;                    /* key head; the row among its sequence's */
     CacheSequence s;
     int pieces = 1, slot0 = unit;
-    if (p.mode == CACHED_TILES) {
+    if constexpr (TILES) {
         const int tile = unit / kv;
         head = unit - tile * kv;
         const auto tiles = [&](int n) { return (long long)((cache_sequence(p.c, p.seq0 + n).fresh * p.per + p.rows - 1) / p.rows); };
@@ -53,11 +58,11 @@ attention_join_kernel(const JoinParams j)
     }
     if (inSeq >= s.fresh * p.per)
         return;
-    const int t = divided(inSeq, p.perDiv), dh = p.c.dh;
+    const int t = divided(inSeq, p.perDiv);
 
     /* the prefix's launch counts rows from the first token of the first sequence */
     int preSlot = 0, preRow = 0, pre = 0;
-    if (j.preAcc) {
+    if (!TILES && j.preAcc) {
         const int start0 = cache_sequence(p.c, p.seq0).start;
         const int fromStart = s.start - start0 + t;
         if (fromStart >= 0 && fromStart < prefix_tokens(p, start0)) {
@@ -69,21 +74,21 @@ attention_join_kernel(const JoinParams j)
         }
     }
 
-    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, col = 4 * lane;
     float mx = -INFINITY, sum = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     constexpr int AHEAD = 4;            /* pieces of a group in flight */
-    for (int i0 = group; i0 < pre + pieces; i0 += 8 * AHEAD) {
+    constexpr int STEP = TILES ? 1 : 8;
+    for (int i0 = TILES ? 0 : group; i0 < pre + pieces; i0 += STEP * AHEAD) {
         float m[AHEAD], l[AHEAD];
         f32x4 x[AHEAD];
         float newMax = mx;
 #pragma unroll
         for (int e = 0; e < AHEAD; e++) {
-            const int i = min(i0 + 8 * e, pre + pieces - 1);
+            const int i = min(i0 + STEP * e, pre + pieces - 1);
             const bool own = i >= pre;
             const long long at = own ? (long long)(slot0 + i - pre) * p.rows + row : (long long)(preSlot + i) * j.preRows + preRow;
             const float * st = (own ? p.stat : j.preStat) + 2 * at;
-            const bool there = i0 + 8 * e < pre + pieces;
+            const bool there = i0 + STEP * e < pre + pieces;
             m[e] = there ? st[0] : -INFINITY;
             l[e] = there ? st[1] : 0.f;
             x[e] = there && col < dh ? *reinterpret_cast<const f32x4 *>((own ? p.acc : j.preAcc) + at * dh + col) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -103,46 +108,56 @@ attention_join_kernel(const JoinParams j)
         }
         mx = newMax;
     }
-    if (lane == 0) {
-        partStat[group][0] = mx;
-        partStat[group][1] = sum;
-    }
-    *reinterpret_cast<f32x4 *>(&partAcc[group][col]) = acc;
-    __syncthreads();
-    if (threadIdx.x < 32 && col < dh) {
+    if constexpr (!TILES) {
+        if (lane == 0) {
+            partStat[group][0] = mx;
+            partStat[group][1] = sum;
+        }
+        *reinterpret_cast<f32x4 *>(&partAcc[group][col]) = acc;
+        __syncthreads();
+        if (threadIdx.x >= 32)
+            return;
         float top = partStat[0][0];
 #pragma unroll
         for (int g = 1; g < 8; g++)
             top = fmaxf(top, partStat[g][0]);
         const float shift = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        sum = 0.f;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int g = 0; g < 8; g++) {
             const float f = __builtin_amdgcn_exp2f(partStat[g][0] - shift);
-            total += f * partStat[g][1];
-            o += *reinterpret_cast<const f32x4 *>(&partAcc[g][col]) * f;
+            sum += f * partStat[g][1];
+            acc += *reinterpret_cast<const f32x4 *>(&partAcc[g][col]) * f;
         }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
+    }
+    if (col < dh) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         typedef T vec __attribute__((ext_vector_type(4)));
         vec v;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            v[e] = (T)(o[e] * inv);
+            v[e] = (T)(acc[e] * inv);
         T * out = static_cast<T *>(p.out) + (long long)(s.start + t) * p.oT + (head * p.per + inSeq - t * p.per) * p.oH;
         *reinterpret_cast<vec *>(out + col) = v;
     }
 }
 
+template <typename T>
+int launch_type(const JoinParams & j, long long rows, hipStream_t stream)
+{
+    if (j.p.mode == CACHED_TILES)
+        hipLaunchKernelGGL((attention_join_kernel<T, true>), dim3((unsigned)(rows / 8)), dim3(256), 0, stream, j);
+    else
+        hipLaunchKernelGGL((attention_join_kernel<T, false>), dim3((unsigned)rows), dim3(256), 0, stream, j);
+    return (int)hipGetLastError();
+}
+
 }  // namespace
 
-int launch_attention_join(const JoinParams & j, bool half, int blocks, hipStream_t stream)
+int launch_attention_join(const JoinParams & j, bool half, long long rows, hipStream_t stream)
 {
-    if (half)
-        hipLaunchKernelGGL((attention_join_kernel<half_t>), dim3((unsigned)blocks), dim3(256), 0, stream, j);
-    else
-        hipLaunchKernelGGL((attention_join_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, j);
-    return (int)hipGetLastError();
+    return half ? launch_type<half_t>(j, rows, stream) : launch_type<float>(j, rows, stream);
 }
 
 }  // namespace ntsamd

@@ -159,16 +159,29 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     }
     const float scale2 = score_scale(p);
 
+    /* One unit ahead, but for the widest tiles of the widest heads: their next unit would take the registers of a second
+       workgroup on the CU, which hides more */
+    constexpr bool AHEAD = QR == 1 || DHM < 128;
     UnitData<T, DHM> next;
     int u = sg.u0 + wave;
-    if (u < sg.u1)
-        load(u, page_of(u), next);
-    int page = page_of(u + 4);
+    int page = page_of(u);
+    if (AHEAD) {
+        if (u < sg.u1)
+            load(u, page, next);
+        page = page_of(u + 4);
+    }
     for (; u < sg.u1; u += 4) {
-        const UnitData<T, DHM> d = next;
-        if (u + 4 < sg.u1)
-            load(u + 4, page, next);
-        page = page_of(u + 8);
+        UnitData<T, DHM> d;
+        if (AHEAD) {
+            d = next;
+            if (u + 4 < sg.u1)
+                load(u + 4, page, next);
+            page = page_of(u + 8);
+        }
+        else {
+            load(u, page, d);
+            page = page_of(u + 4);
+        }
 
         /* ---- S^T = K Q^T ---- */
         f32x4 s[QR][U::NJ];

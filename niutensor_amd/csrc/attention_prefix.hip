@@ -15,7 +15,7 @@ namespace {
 
 /* TILE: rows of a tile of the prefix (16 and 32 float, 64 and 128 half); QR: blocks of 16 rows of a sequence's own */
 template <typename T, int DHM, int TILE, int QR>
-__global__ void __launch_bounds__(256, DHM == 128 && (QR == 2 || TILE == 32) ? 1 : 2)
+__global__ void __launch_bounds__(256, 2)
 attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preBlocks, int ownBlocks)
 {
     __shared__ union Shared {

@@ -1028,6 +1028,21 @@ int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, Ca
     return NTSAMD_OK;
 }
 
+/* Run time of a cached attention in tiles, in microseconds, fitted to graph-replayed calls on 32 to 1024 workgroups, heads of
+   32, 64 and 128 and 1024 and 4096 keys: a workgroup alone on its CU takes `alone` for every 64 keys, and 256 CUs take `busy` for 64
+   keys of every 256 workgroups where more of them share a CU. Tiles of fewer rows read the keys more often and take fewer
+   rows per MFMA's keys, but there are more of them. Keys cut into pieces: as many workgroups for fewer keys, a join (4 us), and their
+   partial rows across memory and back. */
+double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long long keys, int pieces, long long rows)
+{
+    static const double alone[2][2][3] = {{{0.80, 1.15, 1.73}, {1.15, 1.76, 3.0}}, {{0.76, 0.96, 1.40}, {1.07, 1.28, 1.85}}};
+    static const double busy[2][2][3] = {{{0.55, 0.88, 1.5}, {0.85, 1.4, 2.9}}, {{0.38, 0.53, 0.90}, {0.63, 0.88, 1.25}}};
+    const int big = tile == (half ? 128 : 32) ? 1 : 0, width = dh <= 32 ? 0 : (dh <= 64 ? 1 : 2);
+    const double a = alone[half ? 1 : 0][big][width], b = busy[half ? 1 : 0][big][width] * (double)workgroups * pieces / 256.0;
+    const double blocks = (double)((keys + 63) / 64 + pieces - 1) / pieces;
+    return blocks * (a > b ? a : b) + (pieces > 1 ? 4.0 + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 3.0e6 : 0.0);
+}
+
 /* How the rows and keys of a cached attention are dealt out (see attention_cached.hip for the forms). */
 constexpr int CACHED_UNIT_HALF = 32, CACHED_UNIT_FLOAT = 16;
 
@@ -1042,9 +1057,6 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     const long long slotRow = (long long)(dh + 2) * 4;              /* bytes of a partial row */
     const bool mayHold = tuning().splitK.load(std::memory_order_relaxed) != 1;
     const auto units = [unit](long long keys) { return (keys + unit - 1) / unit; };
-    /* a tile of rows: up to 32 go to the kernel whose waves take keys of their own, half tiles of more rows to the one
-       that shares keys through LDS */
-    const auto tile_rows = [half](long long r) { return r <= 16 ? 16 : (r <= 32 || !half ? 32 : (r <= 64 ? 64 : 128)); };
     const auto launch = [half, stream](const CachedParams & c, int tile, long long blocks) {
         return tile > 32 ? launch_attention_cached_tiles(c, tile / 64, (int)blocks, stream)
                          : launch_attention_cached(c, half, tile / 16, (int)blocks, stream);
@@ -1060,26 +1072,32 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     prefix = prefix < p.c.maxLength ? prefix : p.c.maxLength;
 
     if (rows > 32) {
-        /* many rows to a sequence: tiles of rows, their keys in one piece where the tiles fill the part */
+        /* many rows to a sequence: tiles of rows and pieces of keys, whatever of both the estimate likes best */
         p.mode = CACHED_TILES;
-        p.rows = tile_rows(rows);
-        const int keys = p.rows > 32 ? CACHED_TILE_KEYS : 4 * unit;      /* that a workgroup takes at a time */
-        const long long perSeq = (rows + p.rows - 1) / p.rows;
-        long long tiles = (long long)p.c.tokens * p.per / p.rows + n;
-        if (!p.c.starts || n * perSeq < tiles)
-            tiles = n * perSeq;
-        long long pieces = 1;
-        if (mayHold && tiles * kv < 2 * cus) {
-            pieces = (2 * cus + tiles * kv - 1) / (tiles * kv);
-            const long long most = (p.c.maxLength + 4 * keys - 1) / (4 * keys), fit = (long long)SPLIT_WORK_BYTES / (tiles * kv * p.rows * slotRow);
-            pieces = pieces < most ? pieces : most;
-            pieces = pieces < fit ? pieces : fit;
-            if (pieces > 1) {
-                work.take_stream(devID, stream);
-                if (work.mem == NULL)
-                    pieces = 1;
+        long long tiles = 0, pieces = 1;
+        double best = -1.0;
+        for (int big = 0; big < 2; big++) {
+            const int tile = half ? (big ? 128 : 64) : (big ? 32 : 16);
+            const long long perSeq = (rows + tile - 1) / tile;
+            long long of = (long long)p.c.tokens * p.per / tile + n;
+            if (!p.c.starts || n * perSeq < of)
+                of = n * perSeq;
+            for (int cut = 1; cut <= 64; cut += cut < 4 ? 1 : cut / 2) {
+                if (cut > 1 && (!mayHold || of * kv * cut > 4 * cus || 2 * CACHED_TILE_KEYS * cut > p.c.maxLength ||
+                                of * kv * tile * cut * slotRow > (long long)SPLIT_WORK_BYTES))
+                    break;
+                const double t = cached_tiles_cost(half, dh, tile, of * kv, p.c.maxLength, cut, of * kv * tile);
+                if (best < 0.0 || t < best) {
+                    best = t;
+                    tiles = of;
+                    pieces = cut;
+                    p.rows = tile;
+                }
             }
-            else
+        }
+        if (pieces > 1) {
+            work.take_stream(devID, stream);
+            if (work.mem == NULL)
                 pieces = 1;
         }
         if (tiles * kv * pieces > 0x7fffffffLL || (pieces > 1 && tiles * kv * p.rows > 0x7fffffffLL))
@@ -1099,11 +1117,11 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             JoinParams j;
             memset(&j, 0, sizeof(j));
             j.p = p;
-            rc = launch_attention_join(j, half, (int)(tiles * kv * p.rows), stream);
+            rc = launch_attention_join(j, half, tiles * kv * p.rows, stream);
         }
     }
     else {
-        const int tile = tile_rows(rows);
+        const int tile = rows <= 16 ? 16 : 32;
         p.rows = (int)rows;
         const long long room = (long long)SPLIT_WORK_BYTES / slotRow;       /* partial rows that fit */
         const bool shared = prefix >= 4 * unit && n > 1 && mayHold && 512LL * kv <= room;
@@ -1193,7 +1211,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                     j.prePieces = pre.groups;
                     j.preRows = pre.rows;
                 }
-                rc = launch_attention_join(j, half, (int)(pairs * rows), stream);
+                rc = launch_attention_join(j, half, pairs * rows, stream);
             }
         }
     }
