@@ -106,12 +106,12 @@ int ntsamd_attention_cached(int devID, void * stream, const ntsamd_cache * cache
 
 /*
  * ntsamd_attention_cached for sequences that begin alike: the first `prefix` positions of every sequence hold the same
- * keys and values, most often because the first entries of every row of the page table are the same pages. They
- * are read through the first row of the table, once for all sequences: the queries of all sequences are multiplied
+ * keys and values, and are found through the first row of the page table for all of them (what the other rows have
+ * there is not looked at). They are read once for all sequences: the queries of all sequences are multiplied
  * with them as the rows of one matrix; what follows the prefix is read sequence by sequence, and the two partial
  * results are joined. The result is that of ntsamd_attention_cached but for the order of the additions. A sequence
  * shorter than the prefix sees the part of it that it has. Where there is nothing to gain (one sequence, many new
- * tokens per sequence, a short prefix, no workspace) the call runs as ntsamd_attention_cached.
+ * tokens per sequence, a short prefix, no workspace) every sequence reads the prefix for itself.
  */
 int ntsamd_attention_prefix(int devID, void * stream, const ntsamd_cache * cache, const ntsamd_cache_batch * batch,
                             const void * q, void * out, int heads, const long long * strides,

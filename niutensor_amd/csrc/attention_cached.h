@@ -293,7 +293,7 @@ __device__ __forceinline__ long long lane_of(long long x, int source)
     return ((long long)hi << 32) | (unsigned)lo;
 }
 
-/* entry i of a row of the page table: a scalar base and a 32-bit offset (rows are below 4 GiB) */
+/* entry i of a row of the page table (rows are below 4 GiB) */
 __device__ __forceinline__ int page_entry(const int * row, int i)
 {
     return *(const __attribute__((address_space(1))) int *)((const __attribute__((address_space(1))) char *)row + (unsigned)i * 4u);

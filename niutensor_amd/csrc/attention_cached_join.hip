@@ -13,20 +13,19 @@ namespace ntsamd {
 
 namespace {
 
-/* TILES: the rows of tiles of one launch, every one in the same few pieces: eight rows to a workgroup, a group of lanes each.
-   Otherwise a row to a workgroup. */
-template <typename T, bool TILES>
+/* TILES: the rows of a CACHED_TILES launch. MANY: eight rows to a workgroup, a group of lanes each, otherwise a row to a
+   workgroup. */
+template <typename T, bool TILES, bool MANY>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(const JoinParams j)
 {
     __shared__ CachedScan sh;
-    __shared__ float partAcc[TILES ? 1 : 8][128], partStat[8][2];
+    __shared__ float partAcc[MANY ? 1 : 8][128], partStat[8][2];
     const CachedParams & p = j.p;
     const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, col = 4 * lane;
     const int kv = p.c.kvHeads, dh = p.c.dh;
-    /* tiles have multiples of 8 rows: those of a workgroup are of one tile */
-    const int first = (int)blockIdx.x * (TILES ? 8 : 1), id = TILES ? first + group : first;
-    const int unit = first / p.rows, row = id - unit * p.rows;  /* a pair or a tile, and a row of it */
+    const int id = MANY ? (int)blockIdx.x * 8 + group : (int)blockIdx.x;
+    const int unit = id / p.rows, row = id - unit * p.rows;     /* a pair or a tile, and a row of it */
     int head, inSeq;                    /* key head; the row among its sequence's */
     CacheSequence s;
     int pieces = 1, slot0 = unit;
@@ -46,6 +45,8 @@ attention_join_kernel(const JoinParams j)
     }
     else {
         const int i = unit / kv;
+        if (MANY && i >= p.seqs)
+            return;
         head = unit - i * kv;
         s = cache_sequence(p.c, p.seq0 + i);
         inSeq = row;
@@ -77,8 +78,8 @@ attention_join_kernel(const JoinParams j)
     float mx = -INFINITY, sum = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     constexpr int AHEAD = 4;            /* pieces of a group in flight */
-    constexpr int STEP = TILES ? 1 : 8;
-    for (int i0 = TILES ? 0 : group; i0 < pre + pieces; i0 += STEP * AHEAD) {
+    constexpr int STEP = MANY ? 1 : 8;
+    for (int i0 = MANY ? 0 : group; i0 < pre + pieces; i0 += STEP * AHEAD) {
         float m[AHEAD], l[AHEAD];
         f32x4 x[AHEAD];
         float newMax = mx;
@@ -108,7 +109,7 @@ attention_join_kernel(const JoinParams j)
         }
         mx = newMax;
     }
-    if constexpr (!TILES) {
+    if constexpr (!MANY) {
         if (lane == 0) {
             partStat[group][0] = mx;
             partStat[group][1] = sum;
@@ -146,10 +147,14 @@ attention_join_kernel(const JoinParams j)
 template <typename T>
 int launch_type(const JoinParams & j, long long rows, hipStream_t stream)
 {
+    /* Tiles have whole eights of rows, each in the same few pieces. Pairs: few pieces are known of those whose keys are whole. */
+    const dim3 one((unsigned)rows), eight((unsigned)((rows + 7) / 8)), block(256);
     if (j.p.mode == CACHED_TILES)
-        hipLaunchKernelGGL((attention_join_kernel<T, true>), dim3((unsigned)(rows / 8)), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL((attention_join_kernel<T, true, true>), eight, block, 0, stream, j);
+    else if (j.p.mode == CACHED_WHOLE && j.prePieces < 16 && rows >= 2048)
+        hipLaunchKernelGGL((attention_join_kernel<T, false, true>), eight, block, 0, stream, j);
     else
-        hipLaunchKernelGGL((attention_join_kernel<T, false>), dim3((unsigned)rows), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL((attention_join_kernel<T, false, false>), one, block, 0, stream, j);
     return (int)hipGetLastError();
 }
 

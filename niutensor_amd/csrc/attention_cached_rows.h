@@ -90,34 +90,12 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     const int m = lane & 15, g = lane >> 4;
     const int dh = c.dh;
 
-    /* ---- this lane's query rows: positions each sees, fragments ---- */
-    int seen[QR];
-    const int seenMin = rows_seen<QR, 4096>(p, sg, sg.row0 + m, reinterpret_cast<int *>(&sh.acc[0][0][0]), seen);
-    typename U::KPiece qf[QR][U::NT];
-#pragma unroll
-    for (int q = 0; q < QR; q++) {
-        const int row = sg.row0 + 16 * q + m;
-        const bool there = row < sg.rows;
-        const int t = there ? divided(row, p.perDiv) : 0;
-        const int h = sg.head * p.per + (there ? row - t * p.per : 0);
-        const T * qr = static_cast<const T *>(p.q) + (long long)(sg.s.start + t) * p.qT + h * p.qH;
-#pragma unroll
-        for (int t4 = 0; t4 < U::NT; t4++) {
-            constexpr int W = sizeof(typename U::KPiece) / sizeof(T);
-            const int col = 4 * W * t4 + W * g;
-            typename U::KPiece z = {};
-            qf[q][t4] = there && col < dh ? *reinterpret_cast<const typename U::KPiece *>(qr + col) : z;
-            if (p.scale < 0.f)
-                qf[q][t4] = -qf[q][t4];
-        }
-    }
-
     /* ---- loading a unit ---- */
     const int * table = c.table + (long long)sg.seq * c.tablePages;
     const int myKey = lane & (U::UK - 1);
     auto page_of = [&](int u) {
         const int key = p.first + u * U::UK + myKey;
-        return u < sg.u1 && key < sg.keys ? page_entry(table, divided(key, c.pageSize)) : -1;
+        return u < sg.u1 && key < sg.keys ? page_entry(key < p.common ? c.table : table, divided(key, c.pageSize)) : -1;
     };
     /* byte offsets of a lane's columns in a row. Columns past dh read the row's first: a key's meet zeros of q, a value's
        end in columns of the result that are not stored */
@@ -147,6 +125,40 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
         }
     };
 
+    /* One unit ahead, but for the widest tiles of the widest heads: their next unit would take the registers of a second
+       workgroup on the CU, which hides more */
+    constexpr bool AHEAD = QR == 1 || DHM < 128;
+    UnitData<T, DHM> next;
+    int u = sg.u0 + wave;
+    int page = page_of(u);
+    if (AHEAD) {
+        if (u < sg.u1)
+            load(u, page, next);
+        page = page_of(u + 4);
+    }
+
+    /* ---- this lane's query rows: positions each sees, fragments ---- */
+    int seen[QR];
+    const int seenMin = rows_seen<QR, 4096>(p, sg, sg.row0 + m, reinterpret_cast<int *>(&sh.acc[0][0][0]), seen);
+    typename U::KPiece qf[QR][U::NT];
+#pragma unroll
+    for (int q = 0; q < QR; q++) {
+        const int row = sg.row0 + 16 * q + m;
+        const bool there = row < sg.rows;
+        const int t = there ? divided(row, p.perDiv) : 0;
+        const int h = sg.head * p.per + (there ? row - t * p.per : 0);
+        const T * qr = static_cast<const T *>(p.q) + (long long)(sg.s.start + t) * p.qT + h * p.qH;
+#pragma unroll
+        for (int t4 = 0; t4 < U::NT; t4++) {
+            constexpr int W = sizeof(typename U::KPiece) / sizeof(T);
+            const int col = 4 * W * t4 + W * g;
+            typename U::KPiece z = {};
+            qf[q][t4] = there && col < dh ? *reinterpret_cast<const typename U::KPiece *>(qr + col) : z;
+            if (p.scale < 0.f)
+                qf[q][t4] = -qf[q][t4];
+        }
+    }
+
     f32x4 accO[QR][ND];
     float rowMax[QR], rowSum[QR];
 #pragma unroll
@@ -159,17 +171,6 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     }
     const float scale2 = score_scale(p);
 
-    /* One unit ahead, but for the widest tiles of the widest heads: their next unit would take the registers of a second
-       workgroup on the CU, which hides more */
-    constexpr bool AHEAD = QR == 1 || DHM < 128;
-    UnitData<T, DHM> next;
-    int u = sg.u0 + wave;
-    int page = page_of(u);
-    if (AHEAD) {
-        if (u < sg.u1)
-            load(u, page, next);
-        page = page_of(u + 4);
-    }
     for (; u < sg.u1; u += 4) {
         UnitData<T, DHM> d;
         if (AHEAD) {

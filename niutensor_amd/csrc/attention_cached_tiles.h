@@ -66,15 +66,11 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
     const Segment sg = uniform(tile_segment<TR, KB>(p, sh.scan, id));
     if (sg.rows == 0)
         return;
-    const int row0 = sg.row0 + wave * (16 * QR) + m;
-    int seen[QR];
-    const int seenMin = rows_seen<QR, Shared::BLOCK / 4>(p, sg, row0, reinterpret_cast<int *>(sh.k[0]), seen);
-
     /* ---- where the keys of a block stand: lane l looks after key l ---- */
     const int * table = c.table + (long long)sg.seq * c.tablePages;
     auto page_of = [&](int u) {
         const int key = p.first + u * KB + lane;
-        return u < sg.u1 && key < sg.keys ? page_entry(table, divided(key, c.pageSize)) : -1;
+        return u < sg.u1 && key < sg.keys ? page_entry(key < p.common ? c.table : table, divided(key, c.pageSize)) : -1;
     };
     /* the rows that this lane fetches a piece of: row `fetch` + ROWS s of the block */
     const int fetch = wave * (LOADS * ROWS) + lane / PIECES;
@@ -98,10 +94,14 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
         for (int s = 0; s < LOADS; s++)
             lds_from_global16(vLds + stage + s * 1024, lane_of(at.v, fetch + ROWS * s) + col[s]);
     };
-    /* rows_seen may have had numbers in the first stage: every lane is past its last read of them */
+    /* the first block is on its way before anything is asked about the rows */
     if (sg.u0 < sg.u1)
         fetch_block(sg.u0, page_of(sg.u0));
     int page = page_of(sg.u0 + 1);
+
+    const int row0 = sg.row0 + wave * (16 * QR) + m;
+    int seen[QR];
+    const int seenMin = rows_seen<QR, Shared::BLOCK / 4>(p, sg, row0, reinterpret_cast<int *>(sh.k[1]), seen);
 
     /* ---- Q fragments ---- */
     f16x8 qf[QR][NT];

@@ -92,6 +92,7 @@ struct CachedParams {
     int causal;
     int seq0, seqs;                     /* the sequences of this launch: seq0 .. seq0 + seqs - 1 */
     int first;                          /* positions before this one are another launch's (the shared prefix) */
+    int common;                         /* positions before this one are found through the first row of the table */
     int prefix;                         /* > 0: this launch is the shared prefix of that many positions */
     int mode;                           /* CachedMode */
     int groups;                         /* CACHED_PIECES: pieces aimed at; CACHED_TILES: pieces of a tile's keys */

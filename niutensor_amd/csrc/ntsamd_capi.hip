@@ -1031,16 +1031,16 @@ int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, Ca
 /* Run time of a cached attention in tiles, in microseconds, fitted to graph-replayed calls on 32 to 1024 workgroups, heads of
    32, 64 and 128 and 1024 and 4096 keys: a workgroup alone on its CU takes `alone` for every 64 keys, and 256 CUs take `busy` for 64
    keys of every 256 workgroups where more of them share a CU. Tiles of fewer rows read the keys more often and take fewer
-   rows per MFMA's keys, but there are more of them. Keys cut into pieces: as many workgroups for fewer keys, a join (4 us), and their
-   partial rows across memory and back. */
-double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long long keys, int pieces, long long rows)
+   rows per MFMA's keys, but there are more of them. Keys cut into pieces: as many workgroups for fewer keys, a join (`join` us), and their
+   partial rows written and read (about 6 TB/s, most of it behind the multiplications). */
+double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long long keys, int pieces, long long rows, double join)
 {
     static const double alone[2][2][3] = {{{0.80, 1.15, 1.73}, {1.15, 1.76, 3.0}}, {{0.76, 0.96, 1.40}, {1.07, 1.28, 1.85}}};
     static const double busy[2][2][3] = {{{0.55, 0.88, 1.5}, {0.85, 1.4, 2.9}}, {{0.38, 0.53, 0.90}, {0.63, 0.88, 1.25}}};
     const int big = tile == (half ? 128 : 32) ? 1 : 0, width = dh <= 32 ? 0 : (dh <= 64 ? 1 : 2);
     const double a = alone[half ? 1 : 0][big][width], b = busy[half ? 1 : 0][big][width] * (double)workgroups * pieces / 256.0;
     const double blocks = (double)((keys + 63) / 64 + pieces - 1) / pieces;
-    return blocks * (a > b ? a : b) + (pieces > 1 ? 4.0 + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 3.0e6 : 0.0);
+    return blocks * (a > b ? a : b) + (pieces > 1 ? join + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 6.0e6 : 0.0);
 }
 
 /* How the rows and keys of a cached attention are dealt out (see attention_cached.hip for the forms). */
@@ -1070,6 +1070,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     p.prefix = 0;
     p.acc = p.stat = NULL;
     prefix = prefix < p.c.maxLength ? prefix : p.c.maxLength;
+    p.common = prefix;
 
     if (rows > 32) {
         /* many rows to a sequence: tiles of rows and pieces of keys, whatever of both the estimate likes best */
@@ -1086,7 +1087,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 if (cut > 1 && (!mayHold || of * kv * cut > 4 * cus || 2 * CACHED_TILE_KEYS * cut > p.c.maxLength ||
                                 of * kv * tile * cut * slotRow > (long long)SPLIT_WORK_BYTES))
                     break;
-                const double t = cached_tiles_cost(half, dh, tile, of * kv, p.c.maxLength, cut, of * kv * tile);
+                const double t = cached_tiles_cost(half, dh, tile, of * kv, p.c.maxLength, cut, of * kv * tile, 4.0);
                 if (best < 0.0 || t < best) {
                     best = t;
                     tiles = of;
@@ -1124,14 +1125,21 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         const int tile = rows <= 16 ? 16 : 32;
         p.rows = (int)rows;
         const long long room = (long long)SPLIT_WORK_BYTES / slotRow;       /* partial rows that fit */
-        const bool shared = prefix >= 4 * unit && n > 1 && mayHold && 512LL * kv <= room;
-        if (shared || (mayHold && units(p.c.maxLength) > 8))
+        /* keys in pieces, unless they are few, or no more than eight turns of a workgroup's waves and the pairs fill the part */
+        const bool filled = (long long)n * kv >= 2 * cus;
+        const auto many = [filled, units](long long keys) { return units(keys) > (filled ? 32 : 8); };
+        /* A shared prefix costs a join: it pays where the keys would be in pieces, and joined, without it, or where it saves more than
+           64 MB of reading (67 sequences of 286 positions, 256 in common, 8 key heads of 64, half: 13.1 us shared, 8.9 not;
+           49 of 5872, 5864 in common, 8 of 96: 24 and 84). */
+        const long long saved = (long long)(n - 1) * prefix * kv * dh * 2 * (half ? 2 : 4);
+        const bool shared = prefix >= 64 && n > 1 && mayHold && 512LL * kv <= room && (many(p.c.maxLength) || saved > (64 << 20));
+        if (shared || (mayHold && many(p.c.maxLength)))
             work.take_stream(devID, stream);
         const bool withPrefix = shared && work.mem != NULL;
         if (!withPrefix)
             prefix = 0;
         const long long own = p.c.maxLength - prefix;
-        const bool cut = work.mem != NULL && units(own) > 8;
+        const bool cut = work.mem != NULL && many(own);
         /* with a prefix every row has a partial result of its own keys beside those of the prefix's pieces */
         int step = n;
         if (withPrefix) {
@@ -1155,14 +1163,20 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 pre.prefix = prefix;
                 pre.rows = half ? (all <= 64 ? 64 : 128) : (all <= 16 ? 16 : 32);
                 pre.tiles = (int)((all + pre.rows - 1) / pre.rows);
-                /* one workgroup to a CU beside those of the sequences' own keys, two if there are few of these; at least a
-                   round of keys each */
-                const long long slots = (long long)pre.tiles * kv, keys = half ? CACHED_TILE_KEYS : 4 * unit;
-                long long pieces = ((pairs < cus / 2 ? 2 : 1) * cus + slots - 1) / slots;
-                const long long most = (prefix + keys - 1) / keys, fit = room / 2 / (slots * pre.rows);
-                pieces = pieces < most ? pieces : most;
-                pieces = pieces < fit ? pieces : fit;
-                pre.groups = (int)(pieces < 1 ? 1 : pieces);
+                /* pieces of its keys by the estimate for tiles, which is without the sequences' own keys */
+                const long long slots = (long long)pre.tiles * kv;
+                long long pieces = 1;
+                double best = -1.0;
+                for (int of = 1; of <= 64; of += of < 4 ? 1 : of / 4) {
+                    if (of > 1 && (slots * of > 2 * cus || CACHED_TILE_KEYS * of > prefix || slots * pre.rows * of > (cut ? room / 2 : room - pairs * rows)))
+                        break;
+                    const double t = cached_tiles_cost(half, dh, pre.rows, slots, prefix, of, slots * pre.rows, 0.0);
+                    if (best < 0.0 || t < best) {
+                        best = t;
+                        pieces = of;
+                    }
+                }
+                pre.groups = (int)pieces;
                 preBlocks = slots * pre.groups;
                 used = preBlocks * pre.rows;
                 pre.acc = work.mem;
