@@ -359,7 +359,7 @@ class KVCache:
         if k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
             raise NtsAmdError("the columns of the cache must be contiguous")
         self.k, self.v = k, v
-        self.dtype, self.device, self.heads, self.dh = k.dtype, k.device, int(k.shape[2]), int(k.shape[3])
+        self.dtype, self.device, self.heads, self.dh = k.dtype, k.get_device(), int(k.shape[2]), int(k.shape[3])
         self._c = _Cache(k.data_ptr(), v.data_ptr(), _dtype_code(k), k.shape[0], k.shape[1], k.shape[2], k.shape[3],
                          (C.c_longlong * 6)(*k.stride()[:3], *v.stride()[:3]))
         self._ref = C.addressof(self._c)
@@ -381,22 +381,29 @@ class CacheBatch:
             raise NtsAmdError("Unmatched tensors in the batch!")
         self.tensors = (lengths, page_table, starts)
         self.tokens = n * max_new if tokens is None else int(tokens)
-        self.device = lengths.device
+        self.device = lengths.get_device()
         self._c = _CacheBatch(lengths.data_ptr(), starts.data_ptr() if starts is not None else None, page_table.data_ptr(),
                               n, page_table.shape[1], self.tokens, max_new, max_length)
         self._ref = C.addressof(self._c)
 
 
 def _rows(t, cache, batch, heads):
-    """Token and head strides of a [tokens][heads][dh] tensor of the cache's type, on its device."""
-    if t.dim() != 3 or t.dtype != cache.dtype or t.device != cache.device or batch.device != cache.device:
-        raise NtsAmdError("rows of the cache's data type and device, [tokens][heads][dh], are wanted")
-    n, h, d = t.shape
+    """Strides of a [tokens][heads][dh] tensor of the cache's type, on its device."""
+    if t.dtype is not cache.dtype or t.get_device() != cache.device or batch.device != cache.device:
+        raise NtsAmdError("rows of the cache's data type and device are wanted")
     s = t.stride()
-    if n != batch.tokens or h != heads or d != cache.dh or (s[2] != 1 and d > 1):
+    if t.shape != (batch.tokens, heads, cache.dh) or (s[2] != 1 and cache.dh > 1):
         raise NtsAmdError("Unmatched tensors: %s for %d tokens, %d heads of %d contiguous columns"
                           % (tuple(t.shape), batch.tokens, heads, cache.dh))
-    return s[0], s[1]
+    return s
+
+
+def _stream_of(device):
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device) if device >= 0 else None
+
+
+_Strides4, _Strides8 = C.c_longlong * 4, C.c_longlong * 8
 
 
 def cache_append(cache, batch, k, v, rotation=None, pairs=False, q=None, q_out=None):
@@ -404,41 +411,45 @@ def cache_append(cache, batch, k, v, rotation=None, pairs=False, q=None, q_out=N
     queries to q_out (which may be q), turned by rotation: float [positions][columns / 2][2] of cosine and sine.
     pairs: neighbouring columns are turned together, otherwise column j and j + columns / 2."""
     ks, vs = _rows(k, cache, batch, cache.heads), _rows(v, cache, batch, cache.heads)
-    qs = os_ = (0, 0)
+    qs = os_ = ks
     heads = 0
+    qp = op = rp = None
     if q is not None:
-        heads = int(q.shape[1])
+        if q.dim() != 3 or q_out is None:
+            raise NtsAmdError("Unmatched tensors: queries need a [tokens][heads][dh] result")
+        heads = q.shape[1]
         qs, os_ = _rows(q, cache, batch, heads), _rows(q_out, cache, batch, heads)
+        qp, op = q.data_ptr(), q_out.data_ptr()
     positions = rotated = 0
     if rotation is not None:
         if rotation.dim() != 3 or rotation.shape[2] != 2 or not rotation.is_contiguous() or _dtype_code(rotation) != X_FLOAT \
-                or rotation.device != cache.device:
+                or rotation.get_device() != cache.device:
             raise NtsAmdError("rotation must be a dense float [positions][columns / 2][2] tensor")
-        positions, rotated = int(rotation.shape[0]), 2 * int(rotation.shape[1])
-    rc = load().ntsamd_cache_append(cache.device.index, _stream_ptr(k), cache._ref, batch._ref, k.data_ptr(), v.data_ptr(),
-                                    q.data_ptr() if q is not None else None, q_out.data_ptr() if q is not None else None, heads,
-                                    (C.c_longlong * 8)(*ks, *vs, *qs, *os_),
-                                    rotation.data_ptr() if rotation is not None else None, positions, rotated,
-                                    ROTATE_PAIRS if pairs else ROTATE_HALVES)
-    _check(rc)
+        positions, rotated, rp = rotation.shape[0], 2 * rotation.shape[1], rotation.data_ptr()
+    _check(load().ntsamd_cache_append(cache.device, _stream_of(cache.device), cache._ref, batch._ref, k.data_ptr(), v.data_ptr(),
+                                      qp, op, heads, _Strides8(ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1]),
+                                      rp, positions, rotated, ROTATE_PAIRS if pairs else ROTATE_HALVES))
     return q_out
+
+
+def _attention_rows(cache, batch, q, out):
+    if q.dim() != 3:
+        raise NtsAmdError("Unmatched tensors: queries are [tokens][heads][dh]")
+    heads = q.shape[1]
+    qs, os_ = _rows(q, cache, batch, heads), _rows(out, cache, batch, heads)
+    return (cache.device, _stream_of(cache.device), cache._ref, batch._ref, q.data_ptr(), out.data_ptr(), heads,
+            _Strides4(qs[0], qs[1], os_[0], os_[1]))
 
 
 def attention_cached(cache, batch, q, out, scale, causal=True):
     """out = softmax(scale q k^T) v over each sequence's positions in the cache; q and out [tokens][heads][dh], heads a
     multiple of the cache's. causal: a token sees its own position and those before it, otherwise all of them."""
-    heads = int(q.shape[1])
-    strides = (C.c_longlong * 4)(*_rows(q, cache, batch, heads), *_rows(out, cache, batch, heads))
-    _check(load().ntsamd_attention_cached(cache.device.index, _stream_ptr(q), cache._ref, batch._ref, q.data_ptr(), out.data_ptr(),
-                                          heads, strides, scale, 1 if causal else 0))
+    _check(load().ntsamd_attention_cached(*_attention_rows(cache, batch, q, out), scale, 1 if causal else 0))
     return out
 
 
 def attention_prefix(cache, batch, q, out, scale, prefix, causal=True):
     """attention_cached for sequences whose first `prefix` positions hold the same keys and values, which are read through
     the first row of the page table, once for all sequences."""
-    heads = int(q.shape[1])
-    strides = (C.c_longlong * 4)(*_rows(q, cache, batch, heads), *_rows(out, cache, batch, heads))
-    _check(load().ntsamd_attention_prefix(cache.device.index, _stream_ptr(q), cache._ref, batch._ref, q.data_ptr(), out.data_ptr(),
-                                          heads, strides, scale, 1 if causal else 0, prefix))
+    _check(load().ntsamd_attention_prefix(*_attention_rows(cache, batch, q, out), scale, 1 if causal else 0, prefix))
     return out
