@@ -27,13 +27,13 @@ int launch_dhm(const CachedParams & p, int qr, int blocks, hipStream_t stream)
 
 }  // namespace
 
-int launch_attention_cached_tiles(const CachedParams & p, int qr, int blocks, hipStream_t stream)
+int launch_attention_tiles_f16(const CachedParams & p, int tile, int blocks, hipStream_t stream)
 {
     if (p.c.dh <= 32)
-        return launch_dhm<32>(p, qr, blocks, stream);
+        return launch_dhm<32>(p, tile / 64, blocks, stream);
     if (p.c.dh <= 64)
-        return launch_dhm<64>(p, qr, blocks, stream);
-    return launch_dhm<128>(p, qr, blocks, stream);
+        return launch_dhm<64>(p, tile / 64, blocks, stream);
+    return launch_dhm<128>(p, tile / 64, blocks, stream);
 }
 
 }  // namespace ntsamd

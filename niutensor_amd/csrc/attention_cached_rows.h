@@ -31,7 +31,6 @@
 
 namespace ntsamd {
 
-
 template <typename T, int DHM> struct Unit;
 template <int DHM> struct Unit<half_t, DHM> {
     static constexpr int UK = 32, NJ = 2;               /* keys, blocks of 16 of them */
@@ -56,9 +55,10 @@ template <typename T, int DHM> struct UnitData {
     unsigned there;                                     /* which of its keys exist */
 };
 
-struct CachedShared {
-    float acc[4][16][132];
-    float stat[4][16][2];
+/* NW: waves of a workgroup */
+template <int DHM, int NW> struct CachedShared {
+    float acc[NW][16][DHM + 4];
+    float stat[NW][16][2];
     CachedScan scan;
 };
 
@@ -79,8 +79,8 @@ __device__ __forceinline__ void store_columns(T * row, int col, int dh, const fl
         }
 }
 
-template <typename T, int DHM, int QR>
-__device__ __forceinline__ void attend(const CachedParams & p, const Segment & sg, CachedShared & sh)
+template <typename T, int DHM, int QR, int NW>
+__device__ __forceinline__ void attend(const CachedParams & p, const Segment & sg, CachedShared<DHM, NW> & sh)
 {
     typedef Unit<T, DHM> U;
     constexpr int ND = DHM / 16;
@@ -134,12 +134,12 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     if (AHEAD) {
         if (u < sg.u1)
             load(u, page, next);
-        page = page_of(u + 4);
+        page = page_of(u + NW);
     }
 
     /* ---- this lane's query rows: positions each sees, fragments ---- */
     int seen[QR];
-    const int seenMin = rows_seen<QR, 4096>(p, sg, sg.row0 + m, reinterpret_cast<int *>(&sh.acc[0][0][0]), seen);
+    const int seenMin = rows_seen<QR, sizeof(sh.acc) / 4>(p, sg, sg.row0 + m, reinterpret_cast<int *>(&sh.acc[0][0][0]), seen);
     typename U::KPiece qf[QR][U::NT];
 #pragma unroll
     for (int q = 0; q < QR; q++) {
@@ -171,17 +171,17 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     }
     const float scale2 = score_scale(p);
 
-    for (; u < sg.u1; u += 4) {
+    for (; u < sg.u1; u += NW) {
         UnitData<T, DHM> d;
         if (AHEAD) {
             d = next;
-            if (u + 4 < sg.u1)
-                load(u + 4, page, next);
-            page = page_of(u + 8);
+            if (u + NW < sg.u1)
+                load(u + NW, page, next);
+            page = page_of(u + 2 * NW);
         }
         else {
             load(u, page, d);
-            page = page_of(u + 4);
+            page = page_of(u + NW);
         }
 
         /* ---- S^T = K Q^T ---- */
@@ -278,7 +278,7 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
         }
     }
 
-    /* ---- the four waves' results, 16 rows at a time. Register r of MFMA v of set h holds column VC (16 h + 4 g + r) + v of
+    /* ---- the waves' results, 16 rows at a time. Register r of MFMA v of set h holds column VC (16 h + 4 g + r) + v of
        the lane's row ---- */
 #pragma unroll
     for (int q = 0; q < QR; q++) {
@@ -296,10 +296,10 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
                     sh.acc[wave][m][U::VC * (16 * h + 4 * g + r) + v] = accO[q][h * U::VC + v][r];
         __syncthreads();
         const int mine = tid >> 4, col = (tid & 15) * ND, row = sg.row0 + 16 * q + mine;
-        if (row < sg.rows) {
+        if ((NW == 4 || tid < 256) && row < sg.rows) {
             float mx = sh.stat[0][mine][0];
 #pragma unroll
-            for (int w = 1; w < 4; w++)
+            for (int w = 1; w < NW; w++)
                 mx = fmaxf(mx, sh.stat[w][mine][0]);
             const float shift = mx == -INFINITY ? 0.f : mx;
             float total = 0.f, o[ND];
@@ -307,7 +307,7 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
             for (int e = 0; e < ND; e++)
                 o[e] = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < NW; w++) {
                 const float f = __builtin_amdgcn_exp2f(sh.stat[w][mine][0] - shift);
                 total += f * sh.stat[w][mine][1];
 #pragma unroll
@@ -378,20 +378,20 @@ __device__ __forceinline__ Segment pair_segment(const CachedParams & p, CachedSc
 
 /* workgroup `id` of a CACHED_TILES launch, tiles of 16 QR rows */
 template <typename T, int DHM, int QR>
-__device__ __forceinline__ void attend_tile_rows(const CachedParams & p, int id, CachedShared & sh)
+__device__ __forceinline__ void attend_tile_rows(const CachedParams & p, int id, CachedShared<DHM, 4> & sh)
 {
     const Segment sg = uniform(tile_segment<16 * QR, Unit<T, DHM>::UK>(p, sh.scan, id));
     if (sg.rows > 0)
-        attend<T, DHM, QR>(p, sg, sh);
+        attend<T, DHM, QR, 4>(p, sg, sh);
 }
 
-/* workgroup `id` of a CACHED_WHOLE or CACHED_PIECES launch */
-template <typename T, int DHM, int QR>
-__device__ __forceinline__ void attend_pair(const CachedParams & p, int id, CachedShared & sh)
+/* workgroup `id` of a CACHED_WHOLE or CACHED_PIECES launch, NW waves (more than 4: CACHED_WHOLE only, scans take 256 threads) */
+template <typename T, int DHM, int QR, int NW>
+__device__ __forceinline__ void attend_pair(const CachedParams & p, int id, CachedShared<DHM, NW> & sh)
 {
     const Segment sg = uniform(pair_segment<Unit<T, DHM>::UK>(p, sh.scan, id));
     if (sg.rows > 0)
-        attend<T, DHM, QR>(p, sg, sh);
+        attend<T, DHM, QR, NW>(p, sg, sh);
 }
 
 }  // namespace ntsamd

@@ -19,7 +19,7 @@ __global__ void __launch_bounds__(256, 2)
 attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preBlocks, int ownBlocks)
 {
     __shared__ union Shared {
-        CachedShared rows;
+        CachedShared<DHM, 4> rows;
         CachedTilesShared<DHM> tiles;
         __device__ Shared() {}
     } sh;
@@ -43,7 +43,7 @@ attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preB
             attend_tile_rows<T, DHM, TILE / 16>(pre, at, sh.rows);
     }
     else
-        attend_pair<T, DHM, QR>(own, at, sh.rows);
+        attend_pair<T, DHM, QR, 4>(own, at, sh.rows);
 }
 
 template <typename T, int DHM, int TILE>

@@ -1043,6 +1043,23 @@ double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long
     return blocks * (a > b ? a : b) + (pieces > 1 ? join + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 6.0e6 : 0.0);
 }
 
+/* Whether long keys of few rows are better left whole, a workgroup of as many waves as a CU runs to each pair, than cut into pieces
+   that a second kernel joins. Fitted to graph-replayed calls on 8 to 256 pairs, 256 to 4096 keys, all lengths alike and evenly
+   spread: whole, the longest pair's turns of all waves one after the other, slower the more CUs stream; in pieces, a fixed time
+   and the bytes (0.6 of what all pairs would have at the bound) at 5 TB/s. 32 x 8 pairs of 64 columns, lengths to 1021, float:
+   24.6 us in pieces, 21.8 whole; 16 x 8 of 128, 512 keys, half: 14.5 and 10.4, 4096 keys: 57.6 and 61. More pairs than CUs: pieces. */
+bool cached_wide_pays(bool half, int dh, long long pairs, long long keys, int cus)
+{
+    static const double turn[2][3] = {{1.85, 3.6, 3.2}, {1.47, 2.65, 2.4}}, fixed[2][3] = {{4.5, 5.3, 5.0}, {3.8, 4.2, 4.0}};
+    static const double cut[2][3] = {{9.3, 9.8, 11.0}, {9.0, 9.5, 9.5}};
+    const int width = dh <= 32 ? 0 : (dh <= 64 ? 1 : 2), h = half ? 1 : 0;
+    if (pairs > cus)
+        return false;
+    const int each = (half ? 32 : 16) * (dh > 64 ? 8 : 16);         /* keys that a workgroup's waves take in a turn */
+    const double whole = fixed[h][width] + (double)((keys + each - 1) / each) * turn[h][width] * (1.0 + (double)pairs / 1024.0);
+    return whole < cut[h][width] + 0.6 * (double)pairs * (double)keys * dh * 2 * (half ? 2 : 4) / 5.0e6;
+}
+
 /* How the rows and keys of a cached attention are dealt out (see attention_cached.hip for the forms). */
 constexpr int CACHED_UNIT_HALF = 32, CACHED_UNIT_FLOAT = 16;
 
@@ -1057,11 +1074,6 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     const long long slotRow = (long long)(dh + 2) * 4;              /* bytes of a partial row */
     const bool mayHold = tuning().splitK.load(std::memory_order_relaxed) != 1;
     const auto units = [unit](long long keys) { return (keys + unit - 1) / unit; };
-    const auto launch = [half, stream](const CachedParams & c, int tile, long long blocks) {
-        return tile > 32 ? launch_attention_cached_tiles(c, tile / 64, (int)blocks, stream)
-                         : launch_attention_cached(c, half, tile / 16, (int)blocks, stream);
-    };
-    const auto tile_kernel = [](int tile) { return tile > 32 ? "attention_cached_tiles_kernel" : "attention_cached_kernel"; };
     WorkHold work;
     int rc = 0;
     p.seq0 = 0;
@@ -1109,11 +1121,11 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             p.acc = work.mem;
             p.stat = p.acc + tiles * kv * pieces * p.rows * dh;
         }
-        snprintf(g_plan, sizeof(g_plan), "%s tiles=%lldx%d pieces=%lld%s", tile_kernel(p.rows), tiles, p.rows, pieces,
+        snprintf(g_plan, sizeof(g_plan), "%s tiles=%lldx%d pieces=%lld%s", half ? "attention_cached_tiles_kernel" : "attention_cached_tile_kernel", tiles, p.rows, pieces,
                  pieces > 1 ? "+attention_join_kernel" : "");
         if (g_planOnly)
             return NTSAMD_OK;
-        rc = launch(p, p.rows, tiles * kv * pieces);
+        rc = launch_attention_tiles(p, half, p.rows, (int)(tiles * kv * pieces), stream);
         if (rc == 0 && pieces > 1) {
             JoinParams j;
             memset(&j, 0, sizeof(j));
@@ -1133,7 +1145,8 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
            49 of 5872, 5864 in common, 8 of 96: 24 and 84). */
         const long long saved = (long long)(n - 1) * prefix * kv * dh * 2 * (half ? 2 : 4);
         const bool shared = prefix >= 64 && n > 1 && mayHold && 512LL * kv <= room && (many(p.c.maxLength) || saved > (64 << 20));
-        if (shared || (mayHold && many(p.c.maxLength)))
+        const bool wide = !shared && tile == 16 && many(p.c.maxLength) && (mayHold ? cached_wide_pays(half, dh, (long long)n * kv, p.c.maxLength, cus) : (long long)n * kv <= cus);
+        if (shared || (mayHold && many(p.c.maxLength) && !wide))
             work.take_stream(devID, stream);
         const bool withPrefix = shared && work.mem != NULL;
         if (!withPrefix)
@@ -1163,12 +1176,13 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 pre.prefix = prefix;
                 pre.rows = half ? (all <= 64 ? 64 : 128) : (all <= 16 ? 16 : 32);
                 pre.tiles = (int)((all + pre.rows - 1) / pre.rows);
-                /* pieces of its keys by the estimate for tiles, which is without the sequences' own keys */
+                /* pieces of its keys by the estimate for tiles, which is without the sequences' own keys: one workgroup to a CU
+                   beside many of theirs, two beside few */
                 const long long slots = (long long)pre.tiles * kv;
                 long long pieces = 1;
                 double best = -1.0;
                 for (int of = 1; of <= 64; of += of < 4 ? 1 : of / 4) {
-                    if (of > 1 && (slots * of > 2 * cus || CACHED_TILE_KEYS * of > prefix || slots * pre.rows * of > (cut ? room / 2 : room - pairs * rows)))
+                    if (of > 1 && (slots * of > (pairs >= cus / 2 ? 1 : 2) * cus || CACHED_TILE_KEYS * of > prefix || slots * pre.rows * of > (cut ? room / 2 : room - pairs * rows)))
                         break;
                     const double t = cached_tiles_cost(half, dh, pre.rows, slots, prefix, of, slots * pre.rows, 0.0);
                     if (best < 0.0 || t < best) {
@@ -1209,12 +1223,12 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             char text[96] = "attention_cached_kernel";
             if (withPrefix)
                 snprintf(text, sizeof(text), "attention_prefix_kernel tiles=%dx%d pieces=%d", pre.tiles, pre.rows, pre.groups);
-            snprintf(g_plan, sizeof(g_plan), "%s rows=%d %s=%lld%s", text, tile, o.mode == CACHED_PIECES ? "pieces" : "whole", blocks,
+            snprintf(g_plan, sizeof(g_plan), "%s rows=%d %s%s=%lld%s", text, tile, wide ? "wide " : "", o.mode == CACHED_PIECES ? "pieces" : "whole", blocks,
                      o.acc ? "+attention_join_kernel" : "");
             if (g_planOnly)
                 return NTSAMD_OK;
             rc = withPrefix ? launch_attention_prefix(pre, o, half, pre.rows, tile / 16, (int)preBlocks, (int)blocks, stream)
-                            : launch(o, tile, blocks);
+                            : launch_attention_pairs(o, half, tile, wide, (int)blocks, stream);
             if (rc == 0 && o.acc) {
                 JoinParams j;
                 memset(&j, 0, sizeof(j));

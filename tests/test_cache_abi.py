@@ -131,9 +131,11 @@ def test_plans(planning):
     # long ones: in pieces
     assert attend(n=8, tokens=8, width=512) == 0
     assert re.fullmatch(r"attention_cached_kernel rows=16 pieces=\d+\+attention_join_kernel", nt.last_plan())
+    # ones in between, or long ones without a workspace: whole, but by more waves
+    assert attend(n=8, tokens=8, width=32) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 wide whole=16"
     nt.tuning_set("NTSAMD_SPLIT_K", 1)
-    assert attend(n=8, tokens=8, width=512) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 whole=16"
-    assert attend(n=8, tokens=8, width=512, prefix=1024) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 whole=16"
+    assert attend(n=8, tokens=8, width=512) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 wide whole=16"
+    assert attend(n=8, tokens=8, width=512, prefix=1024) == 0 and nt.last_plan() == "attention_cached_kernel rows=16 wide whole=16"
     nt.tuning_set("NTSAMD_SPLIT_K", None)
     # the prefix once for all, each sequence's own keys, and the join
     assert attend(n=8, tokens=8, width=512, prefix=1024) == 0
