@@ -308,9 +308,9 @@ __device__ __forceinline__ V load_global(long long address)
 /* CACHED_WHOLE, CACHED_PIECES: `tile` (16 or 32) rows to a pair at most. wide: CACHED_WHOLE without partial results, up to 16 rows,
    as many waves to a workgroup as a CU runs */
 int launch_attention_pairs(const CachedParams & p, bool half, int tile, bool wide, int blocks, hipStream_t stream);
-/* CACHED_TILES: tiles of 64 or 128 rows (half), 16 or 32 (float) */
+/* CACHED_TILES: tiles of 64 or 128 (half) rows; float tiles of 16 or 32 */
 int launch_attention_tiles(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream);
-int launch_attention_tiles_f16(const CachedParams & p, int tile, int blocks, hipStream_t stream);
+int launch_attention_tile_rows(const CachedParams & p, int tile, int blocks, hipStream_t stream);
 constexpr int CACHED_TILE_KEYS = 64;
 /* both launches of a shared prefix in one: `pre` over it in tiles of `tile` rows (64 or 128 half, 16 or 32 float), `own` over each
    sequence's own keys, 16 qr rows */

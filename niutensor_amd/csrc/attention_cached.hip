@@ -19,7 +19,7 @@ attention_cached_kernel(const CachedParams p)
     attend_pair<T, DHM, QR, NW>(p, (int)blockIdx.x, sh);
 }
 
-/* CACHED_TILES, float (half tiles have more rows: attention_cached_f16.hip) */
+/* CACHED_TILES, float tiles of 16 or 32 rows (more rows, and half: attention_cached_tiles.hip) */
 template <int DHM, int QR>
 __global__ void __launch_bounds__(256, 2)
 attention_cached_tile_kernel(const CachedParams p)
@@ -48,6 +48,9 @@ int launch_type(const CachedParams & p, int tile, bool wide, int blocks, hipStre
         return launch_pairs<T, 32>(p, tile, wide, blocks, stream);
     if (p.c.dh <= 64)
         return launch_pairs<T, 64>(p, tile, wide, blocks, stream);
+    if constexpr (sizeof(T) == 4)
+        if (p.c.dh <= 96)
+            return launch_pairs<T, 96>(p, tile, wide, blocks, stream);
     return launch_pairs<T, 128>(p, tile, wide, blocks, stream);
 }
 
@@ -68,14 +71,14 @@ int launch_attention_pairs(const CachedParams & p, bool half, int tile, bool wid
     return half ? launch_type<half_t>(p, tile, wide, blocks, stream) : launch_type<float>(p, tile, wide, blocks, stream);
 }
 
-int launch_attention_tiles(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream)
+int launch_attention_tile_rows(const CachedParams & p, int tile, int blocks, hipStream_t stream)
 {
-    if (half)
-        return launch_attention_tiles_f16(p, tile, blocks, stream);
     if (p.c.dh <= 32)
         return launch_tile<32>(p, tile, blocks, stream);
     if (p.c.dh <= 64)
         return launch_tile<64>(p, tile, blocks, stream);
+    if (p.c.dh <= 96)
+        return launch_tile<96>(p, tile, blocks, stream);
     return launch_tile<128>(p, tile, blocks, stream);
 }
 

@@ -44,7 +44,7 @@ template <int DHM> struct Unit<float, DHM> {
     static constexpr int UK = 16, NJ = 1;
     static constexpr int NT = DHM / 16;
     static constexpr int NV = 4;
-    static constexpr int VC = DHM >= 64 ? 4 : DHM / 16, NH = DHM / 16 / VC;
+    static constexpr int VC = DHM % 64 == 0 ? 4 : 2, NH = DHM / 16 / VC;
     typedef f32x4 KPiece;
     typedef float VPiece __attribute__((ext_vector_type(VC)));
 };
@@ -66,7 +66,8 @@ template <int DHM, int NW> struct CachedShared {
 template <typename T, int ND>
 __device__ __forceinline__ void store_columns(T * row, int col, int dh, const float (&x)[ND], float f)
 {
-    constexpr int W = ND < 16 / (int)sizeof(T) ? ND : 16 / (int)sizeof(T);      /* dh is a multiple of 16 / sizeof(T) */
+    constexpr int MOST = 16 / (int)sizeof(T);                           /* dh is a multiple of it */
+    constexpr int W = ND < MOST ? ND : (ND % MOST == 0 ? MOST : 2);
     typedef T vec __attribute__((ext_vector_type(W)));
 #pragma unroll
     for (int at = 0; at < ND; at += W)

@@ -22,18 +22,21 @@
 
 namespace ntsamd {
 
-/* Two stages of a block of keys and values. Rows are 2 DHM bytes, without padding (they are written 16 bytes a lane, one
-   lane after the other); which 16-byte piece of a row stands where is swizzled by the row instead, so that 16 rows read
-   at one column, and the pairs of pieces that a transposing read takes of 8 rows, spread over all banks. */
-template <int DHM> struct CachedTilesShared {
-    static constexpr int PIECES = DHM / 8, BLOCK = CACHED_TILE_KEYS * DHM * 2;
+/* Two stages of a block of keys and values: KB keys, 32 KB at most, so that two workgroups share a CU. Rows are those of DHM columns,
+   without padding (they are written 16 bytes a lane, one lane after the other); which 16-byte piece of a row stands where is
+   swizzled by the row instead, so that 16 rows read at one column, and in half the pairs of pieces that a transposing read takes of
+   8 rows, spread over all banks. */
+template <typename T, int DHM> struct CachedTilesShared {
+    static constexpr int KB = sizeof(T) == 4 && DHM > 64 ? 32 : 64;
+    static constexpr int PIECES = DHM * (int)sizeof(T) / 16, ROW = DHM * (int)sizeof(T), BLOCK = KB * ROW;
     __attribute__((aligned(1024))) char k[2][BLOCK];
     __attribute__((aligned(1024))) char v[2][BLOCK];
     CachedScan scan;
     static __device__ __forceinline__ int swizzle(int row)
     {
-        const int k = (row & 15) * PIECES / 16;         /* rows that share the 256 bytes of a round of banks take the same */
-        return ((k & (PIECES / 2 - 1)) << 1) | (k / (PIECES / 2));
+        /* rows that share the 256 bytes of a round of banks take the same */
+        const int k = PIECES >= 16 ? row & 15 : (row & 15) * PIECES / 16;
+        return sizeof(T) == 4 ? k : ((k & (PIECES / 2 - 1)) << 1) | (k / (PIECES / 2));
     }
 };
 
@@ -47,57 +50,94 @@ __device__ __forceinline__ void lds_from_global16(unsigned lds, long long addres
                  : "memory");
 }
 
-/* workgroup `id` of a CACHED_TILES launch over half tensors, tiles of 64 QR rows */
-template <int DHM, int QR>
-__device__ __forceinline__ void attend_tile(const CachedParams & p, int id, CachedTilesShared<DHM> & sh)
-{
-    typedef CachedTilesShared<DHM> Shared;
-    constexpr int KB = CACHED_TILE_KEYS, TR = 64 * QR;
-    constexpr int NT = DHM / 32, ND = DHM / 16, NJ = KB / 16;
-    constexpr int PIECES = Shared::PIECES, ROWS = 64 / PIECES;          /* rows of a block that a wave fetches at a time */
-    constexpr int LOADS = KB / (4 * ROWS);
+/* What fetches a tile's blocks: lane l of every wave looks after key l of a block */
+template <typename T, int DHM> struct TileFetch {
+    typedef CachedTilesShared<T, DHM> Shared;
+    static constexpr int KB = Shared::KB, PIECES = Shared::PIECES;
+    static constexpr int ROWS = 64 / PIECES;            /* rows of a block that a wave fetches at a time */
+    static constexpr int LOADS = KB / (4 * ROWS);
+    const CachedParams & p;
+    const Segment & sg;
+    const int * table;
+    int lane, fetch;                        /* this lane fetches a piece of each of the rows `fetch` + ROWS s */
+    int col[LOADS];                         /* columns past dh: the row's first, which meet zeros of q or are not stored */
+    unsigned kLds, vLds;
+    unsigned long long there;               /* which keys of the block being fetched exist */
+    KeyPlace at;                            /* of the lane's key of that block */
 
-    const CacheParams & c = p.c;
+    __device__ __forceinline__ TileFetch(const CachedParams & params, const Segment & segment, Shared & sh, int wave, int l)
+        : p(params), sg(segment), table(params.c.table + (long long)segment.seq * params.c.tablePages), lane(l),
+          fetch(wave * (LOADS * ROWS) + l / PIECES), there(0)
+    {
+#pragma unroll
+        for (int s = 0; s < LOADS; s++) {
+            const int at = 16 * ((lane % PIECES) ^ Shared::swizzle(fetch + ROWS * s));
+            col[s] = at < (int)sizeof(T) * p.c.dh ? at : 0;
+        }
+        kLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.k[0]) + wave * (LOADS * 1024);
+        vLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.v[0]) + wave * (LOADS * 1024);
+    }
+    /* the page of the lane's key of block u */
+    __device__ __forceinline__ int page_of(int u) const
+    {
+        const int key = p.first + u * KB + lane;
+        return u < sg.u1 && key < sg.keys && (KB == 64 || lane < KB) ? page_entry(key < p.common ? p.c.table : table, divided(key, p.c.pageSize)) : -1;
+    }
+    /* a block's fetch: look(u, ..), then loads 0 .. 2 LOADS - 1, each the address and the load itself */
+    __device__ __forceinline__ void look(int u, int page)
+    {
+        at = key_place<T>(p.c, sg.head, p.first + u * KB + lane, page);
+        there = __ballot(at.there);
+    }
+    __device__ __forceinline__ long long source(int i) const
+    {
+        const int s = i % LOADS;
+        return lane_of(i < LOADS ? at.k : at.v, fetch + ROWS * s) + col[s];
+    }
+    __device__ __forceinline__ void load(int u, int i, long long source) const
+    {
+        lds_from_global16((i < LOADS ? kLds : vLds) + ((u - sg.u0) & 1) * Shared::BLOCK + (i % LOADS) * 1024, source);
+    }
+    __device__ __forceinline__ void block(int u, int page)
+    {
+        look(u, page);
+#pragma unroll
+        for (int i = 0; i < 2 * LOADS; i++)
+            load(u, i, source(i));
+    }
+    /* the block being fetched has landed, for every wave, and nobody reads the other stage any more */
+    __device__ __forceinline__ void landed() const
+    {
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt<0>();
+        wait_lgkmcnt0();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
+/* workgroup `id` of a CACHED_TILES launch over half tensors, tiles of 64 QR rows. DHC: columns computed with, at least dh (rows of 80
+   or 96 columns stand in LDS as rows of 128) */
+template <int DHM, int DHC, int QR>
+__device__ __forceinline__ void attend_tile(const CachedParams & p, int id, CachedTilesShared<half_t, DHM> & sh)
+{
+    typedef CachedTilesShared<half_t, DHM> Shared;
+    constexpr int KB = CACHED_TILE_KEYS, TR = 64 * QR;
+    constexpr int NT = DHC / 32, ND = DHC / 16, NJ = KB / 16;
+
     const int tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, g = lane >> 4;
-    const int dh = c.dh;
+    const int dh = p.c.dh;
 
     const Segment sg = uniform(tile_segment<TR, KB>(p, sh.scan, id));
     if (sg.rows == 0)
         return;
-    /* ---- where the keys of a block stand: lane l looks after key l ---- */
-    const int * table = c.table + (long long)sg.seq * c.tablePages;
-    auto page_of = [&](int u) {
-        const int key = p.first + u * KB + lane;
-        return u < sg.u1 && key < sg.keys ? page_entry(key < p.common ? c.table : table, divided(key, c.pageSize)) : -1;
-    };
-    /* the rows that this lane fetches a piece of: row `fetch` + ROWS s of the block */
-    const int fetch = wave * (LOADS * ROWS) + lane / PIECES;
-    int col[LOADS];                          /* columns past dh: the row's first, which meet zeros of q or are not stored */
-#pragma unroll
-    for (int s = 0; s < LOADS; s++) {
-        const int at = 16 * ((lane % PIECES) ^ Shared::swizzle(fetch + ROWS * s));
-        col[s] = at < 2 * dh ? at : 0;
-    }
-    const unsigned kLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.k[0]) + wave * (LOADS * 1024);
-    const unsigned vLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.v[0]) + wave * (LOADS * 1024);
-    unsigned long long there = 0;            /* which keys of the block being fetched exist */
-    auto fetch_block = [&](int u, int page) {
-        const KeyPlace at = key_place<half_t>(c, sg.head, p.first + u * KB + lane, page);
-        const unsigned stage = ((u - sg.u0) & 1) * Shared::BLOCK;
-        there = __ballot(at.there);
-#pragma unroll
-        for (int s = 0; s < LOADS; s++)
-            lds_from_global16(kLds + stage + s * 1024, lane_of(at.k, fetch + ROWS * s) + col[s]);
-#pragma unroll
-        for (int s = 0; s < LOADS; s++)
-            lds_from_global16(vLds + stage + s * 1024, lane_of(at.v, fetch + ROWS * s) + col[s]);
-    };
+    TileFetch<half_t, DHM> from(p, sg, sh, wave, lane);
     /* the first block is on its way before anything is asked about the rows */
     if (sg.u0 < sg.u1)
-        fetch_block(sg.u0, page_of(sg.u0));
-    int page = page_of(sg.u0 + 1);
+        from.block(sg.u0, from.page_of(sg.u0));
+    int page = from.page_of(sg.u0 + 1);
 
     const int row0 = sg.row0 + wave * (16 * QR) + m;
     int seen[QR];
@@ -148,19 +188,13 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
 
     for (int u = sg.u0; u < sg.u1; u++) {
         const int key0 = p.first + u * KB;
-        const unsigned long long exist = there;
+        const unsigned long long exist = from.there;
         const char * const Ks = sh.k[(u - sg.u0) & 1];
         const char * const Vs = sh.v[(u - sg.u0) & 1];
-        /* this block has landed, for every wave, and nobody reads the other stage any more: it is filled while this one is
-           worked on */
-        __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<0>();
-        wait_lgkmcnt0();
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+        from.landed();
         if (u + 1 < sg.u1)
-            fetch_block(u + 1, page);
-        page = page_of(u + 2);
+            from.block(u + 1, page);
+        page = from.page_of(u + 2);
 
         /* ---- S^T = K Q^T ---- */
         f32x4 accS[QR][NJ];

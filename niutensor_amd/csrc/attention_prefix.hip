@@ -20,7 +20,7 @@ attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preB
 {
     __shared__ union Shared {
         CachedShared<DHM, 4> rows;
-        CachedTilesShared<DHM> tiles;
+        CachedTilesShared<half_t, DHM == 96 ? 32 : DHM> tiles;      /* half only, which has no 96 */
         __device__ Shared() {}
     } sh;
     const int id = (int)blockIdx.x, both = 2 * (min(preBlocks, ownBlocks) & ~7);
@@ -38,7 +38,7 @@ attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preB
     }
     if (first) {
         if constexpr (TILE > 32)
-            attend_tile<DHM, TILE / 64>(pre, at, sh.tiles);
+            attend_tile<DHM, DHM, TILE / 64>(pre, at, sh.tiles);
         else
             attend_tile_rows<T, DHM, TILE / 16>(pre, at, sh.rows);
     }
@@ -61,9 +61,10 @@ template <int DHM>
 int launch_dhm(const CachedParams & pre, const CachedParams & own, bool half, int tile, int qr, int preBlocks, int ownBlocks,
                hipStream_t stream)
 {
-    if (half)
-        return tile <= 64 ? launch_tile<half_t, DHM, 64>(pre, own, qr, preBlocks, ownBlocks, stream)
-                          : launch_tile<half_t, DHM, 128>(pre, own, qr, preBlocks, ownBlocks, stream);
+    if constexpr (DHM != 96)
+        if (half)
+            return tile <= 64 ? launch_tile<half_t, DHM, 64>(pre, own, qr, preBlocks, ownBlocks, stream)
+                              : launch_tile<half_t, DHM, 128>(pre, own, qr, preBlocks, ownBlocks, stream);
     return tile <= 16 ? launch_tile<float, DHM, 16>(pre, own, qr, preBlocks, ownBlocks, stream)
                       : launch_tile<float, DHM, 32>(pre, own, qr, preBlocks, ownBlocks, stream);
 }
@@ -77,6 +78,8 @@ int launch_attention_prefix(const CachedParams & pre, const CachedParams & own, 
         return launch_dhm<32>(pre, own, half, tile, qr, preBlocks, ownBlocks, stream);
     if (pre.c.dh <= 64)
         return launch_dhm<64>(pre, own, half, tile, qr, preBlocks, ownBlocks, stream);
+    if (pre.c.dh <= 96 && !half)
+        return launch_dhm<96>(pre, own, half, tile, qr, preBlocks, ownBlocks, stream);
     return launch_dhm<128>(pre, own, half, tile, qr, preBlocks, ownBlocks, stream);
 }
 

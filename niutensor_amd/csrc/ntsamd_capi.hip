@@ -1028,19 +1028,25 @@ int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, Ca
     return NTSAMD_OK;
 }
 
-/* Run time of a cached attention in tiles, in microseconds, fitted to graph-replayed calls on 32 to 1024 workgroups, heads of
-   32, 64 and 128 and 1024 and 4096 keys: a workgroup alone on its CU takes `alone` for every 64 keys, and 256 CUs take `busy` for 64
-   keys of every 256 workgroups where more of them share a CU. Tiles of fewer rows read the keys more often and take fewer
-   rows per MFMA's keys, but there are more of them. Keys cut into pieces: as many workgroups for fewer keys, a join (`join` us), and their
-   partial rows written and read (about 6 TB/s, most of it behind the multiplications). */
+/* Run time of a cached attention in tiles, in microseconds, fitted to graph-replayed calls on 8 to 2048 workgroups, heads of 32, 64,
+   96 and 128, 1024 to 4096 keys, and to calls of uneven lengths. A workgroup alone on its CU takes `alone` for every 64 keys; 256 CUs
+   take `busy` for 64 keys of every 256 workgroups where more of them share a CU. With more workgroups than CUs it is half of that (of
+   the lengths, about half is there) and most of the longest one's own time. Tiles of fewer rows read the keys more often and take
+   fewer rows per MFMA's keys, but there are more of them, and shorter ones. Keys cut into pieces: as many workgroups for fewer keys, a
+   join (`join` us), and their partial rows written and read (about 6 TB/s, most of it behind the multiplications).
+   Float, 13 pieces of text of up to 784 tokens behind up to 3282, 8 heads of 128 on one key head, tiles of 16, 32, 64 rows: 774,
+   661, 719 us; 45 of 567 of 829, 32 on 8 of 64: 955, 879, 731; 36 of 339 of 2425, 16 on 4 of 96, half, 64 and 128: 176, 134. */
 double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long long keys, int pieces, long long rows, double join)
 {
-    static const double alone[2][2][3] = {{{0.80, 1.15, 1.73}, {1.15, 1.76, 3.0}}, {{0.76, 0.96, 1.40}, {1.07, 1.28, 1.85}}};
-    static const double busy[2][2][3] = {{{0.55, 0.88, 1.5}, {0.85, 1.4, 2.9}}, {{0.38, 0.53, 0.90}, {0.63, 0.88, 1.25}}};
-    const int big = tile == (half ? 128 : 32) ? 1 : 0, width = dh <= 32 ? 0 : (dh <= 64 ? 1 : 2);
-    const double a = alone[half ? 1 : 0][big][width], b = busy[half ? 1 : 0][big][width] * (double)workgroups * pieces / 256.0;
+    static const double alone[5][4] = {{0.87, 1.17, 1.50, 1.75}, {1.27, 1.79, 2.34, 2.80}, {1.72, 2.71, 4.48, 5.43},
+                                       {0.76, 0.96, 1.34, 1.40}, {1.07, 1.28, 1.65, 1.85}};
+    static const double busy[5][4] = {{0.50, 0.85, 1.46, 1.65}, {0.85, 1.45, 2.36, 2.65}, {1.39, 2.39, 3.69, 4.60},
+                                      {0.38, 0.53, 0.85, 0.90}, {0.63, 0.88, 1.15, 1.25}};
+    const int kind = half ? (tile == 64 ? 3 : 4) : (tile == 16 ? 0 : (tile == 32 ? 1 : 2));
+    const int width = dh <= 32 ? 0 : (dh <= 64 ? 1 : (dh <= 96 ? 2 : 3));
+    const double a = alone[kind][width], load = (double)workgroups * pieces / 256.0, b = 0.5 * busy[kind][width] * load + 0.8 * a;
     const double blocks = (double)((keys + 63) / 64 + pieces - 1) / pieces;
-    return blocks * (a > b ? a : b) + (pieces > 1 ? join + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 6.0e6 : 0.0);
+    return blocks * (load <= 1.0 || a > b ? a : b) + (pieces > 1 ? join + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 6.0e6 : 0.0);
 }
 
 /* Whether long keys of few rows are better left whole, a workgroup of as many waves as a CU runs to each pair, than cut into pieces
@@ -1089,8 +1095,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         p.mode = CACHED_TILES;
         long long tiles = 0, pieces = 1;
         double best = -1.0;
-        for (int big = 0; big < 2; big++) {
-            const int tile = half ? (big ? 128 : 64) : (big ? 32 : 16);
+        for (int tile = half ? 64 : 16; tile <= (half ? 128 : 64); tile *= 2) {
             const long long perSeq = (rows + tile - 1) / tile;
             long long of = (long long)p.c.tokens * p.per / tile + n;
             if (!p.c.starts || n * perSeq < of)
@@ -1121,11 +1126,12 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             p.acc = work.mem;
             p.stat = p.acc + tiles * kv * pieces * p.rows * dh;
         }
-        snprintf(g_plan, sizeof(g_plan), "%s tiles=%lldx%d pieces=%lld%s", half ? "attention_cached_tiles_kernel" : "attention_cached_tile_kernel", tiles, p.rows, pieces,
+        snprintf(g_plan, sizeof(g_plan), "%s tiles=%lldx%d pieces=%lld%s", p.rows >= 64 ? "attention_cached_tiles_kernel" : "attention_cached_tile_kernel", tiles, p.rows, pieces,
                  pieces > 1 ? "+attention_join_kernel" : "");
         if (g_planOnly)
             return NTSAMD_OK;
-        rc = launch_attention_tiles(p, half, p.rows, (int)(tiles * kv * pieces), stream);
+        rc = p.rows >= 64 ? launch_attention_tiles(p, half, p.rows, (int)(tiles * kv * pieces), stream)
+                          : launch_attention_tile_rows(p, p.rows, (int)(tiles * kv * pieces), stream);
         if (rc == 0 && pieces > 1) {
             JoinParams j;
             memset(&j, 0, sizeof(j));

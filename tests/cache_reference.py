@@ -6,8 +6,10 @@ Attention, per result element, with p_j the probabilities, A = sum_j p_j |v_j|, 
              a probability and the sum of all by exp(+-2 d): 2 d each on both sides of the quotient -> 4 d A;
   exp2, sums every exp2, its scaled argument (|s| log2 e 2^-24 absolute, twice for the shift), rescaling and addition:
              n + 64 roundings of 2^-24, and 4 |s|max 2^-24 -> (n + 64 + 4 smax) 2^-24 A;
-  half       probabilities rounded to half: 2^-11 A, or 2^-25 each where they are below the normal range: 2^-25 sum |v_j|
-             (the sum they are divided by is at least 1); the result: 2^-11 |out|, 2^-25 at least.
+  half       probabilities, of 2^8 at most before they are divided, rounded to half: 2^-11 A, or 2^-25 each where they are below the
+             normal range: 2^-25 sum |v_j| (the sum they are divided by is at least 1). That sum may be the exact or the rounded
+             ones': in the second case it is off by 2^-11 of itself and n 2^-25, so the result by (2^-11 + n 2^-25) |out| more.
+             The result: 2^-11 |out|, 2^-25 at least.
 """
 import math
 
@@ -121,6 +123,7 @@ class Problem:
                 t = (4 * d + (len(rows) + 64 + 4 * smax) * 2.0 ** -24) * a + 2.0 ** -126
                 if self.half:
                     t = t + 2.0 ** -11 * a + 2.0 ** -25 * ((~hide).double() @ vs.abs()) + torch.maximum(2.0 ** -11 * o.abs(), torch.tensor(2.0 ** -25))
+                    t = t + (2.0 ** -11 + 2.0 ** -25 * seen[:, None]) * o.abs()
                     t = t * (1 + 2.0 ** -10)            # the bounds on each other's results
                 want[self.starts[i]:self.starts[i] + n, h], tol[self.starts[i]:self.starts[i] + n, h] = o, t
         return want, tol

@@ -166,6 +166,61 @@ def test_cached(gpu, lens, new, heads, kv, dh, page, half, causal, layout, unifo
     assert (out == first).all()                                                    # the same bits on every run
 
 
+TILES = [
+    # sequences, positions, new tokens, heads, kv, dh, page, half, causal: the tiles' rows, and whether the keys are in pieces
+    ((3, 70, 40, 64, 8, 80, 16, False, True), 32, False),
+    ((4, 1000, 40, 8, 1, 128, 100, False, True), 32, True),
+    ((8, 130, 120, 64, 8, 32, 20, False, True), 64, False),
+    ((8, 130, 120, 64, 8, 64, 16, False, False), 64, False),
+    ((8, 300, 250, 32, 4, 84, 16, False, True), 64, False),
+    ((8, 300, 250, 64, 8, 128, 7, False, True), 64, False),
+    ((4, 1700, 40, 64, 8, 96, 16, False, True), 64, True),
+    ((3, 70, 40, 64, 8, 96, 16, True, False), 64, False),
+    ((3, 1700, 900, 8, 2, 32, 16, True, True), 128, True),
+    ((8, 70, 64, 64, 8, 64, 20, True, True), 128, False),
+    ((8, 70, 64, 64, 8, 88, 16, True, False), 128, False),
+    ((8, 70, 64, 64, 8, 128, 16, True, True), 128, False),
+    ((8, 1700, 40, 4, 2, 96, 16, True, True), 128, True),
+]
+
+
+@pytest.mark.parametrize("sizes,rows,pieces", TILES)
+def test_every_kind_of_tile(gpu, sizes, rows, pieces):
+    n, size, new, heads, kv, dh, page, half, causal = sizes
+    p = Problem([size - 3 * i for i in range(n)], [new - 2 * i for i in range(n)], heads, kv, dh, page, half, 17,
+                layout="heads" if dh % 32 else "rows", pad_tokens=1)
+    cache, batch, q, out = p.place(nt)
+    want, tol = p.attention(causal)
+    nt.attention_cached(cache, batch, q, out, p.scale, causal=causal)
+    assert "x%d pieces=" % rows in nt.last_plan() and pieces == ("join" in nt.last_plan()), nt.last_plan()
+    assert_within(out, want, tol, nt.last_plan())
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+def test_long_keys_of_few_pairs_by_more_waves(gpu, half, dh):
+    p = Problem([1021, 700, 0, 17, 512], [1] * 5, 6, 2, dh, 20, half, 18, uniform=True)
+    cache, batch, q, out = p.place(nt)
+    want, tol = p.attention(True)
+    nt.tuning_set("NTSAMD_SPLIT_K", 1)
+    nt.attention_cached(cache, batch, q, out, p.scale)
+    assert "wide" in nt.last_plan(), nt.last_plan()
+    assert_within(out, want, tol, nt.last_plan())
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_of_zero_and_below(gpu, half, new, scale):
+    """Zero: the mean of what is seen; below: the smallest products weigh most."""
+    p = Problem([90, 33, 30], [new] * 3, 4, 2, 64, 16, half, 19)
+    p.scale = scale
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_cached(cache, batch, q, out, scale)
+    assert_within(out, want, tol, nt.last_plan())
+
+
 @pytest.mark.parametrize("half", [True, False])
 def test_absent_pages_and_rows_that_see_nothing(gpu, half):
     """Positions on absent pages are left out; a sequence with none left, or more new tokens than positions, gives zeros there."""
