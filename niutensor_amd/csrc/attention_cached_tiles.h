@@ -116,6 +116,23 @@ template <typename T, int DHM> struct TileFetch {
     }
 };
 
+/* Hides from a row's scores of a block those of keys that do not exist and of keys past the `left` ones that the row sees. Register r
+   of part j is key 16 j + 4 g + r. Nothing of it is to be computed where it is not called (the compiler would keep a mask for every
+   register for the whole loop). */
+template <int NJ>
+__device__ __forceinline__ void hide_scores(f32x4 (&s)[NJ], unsigned long long exist, int left, int g)
+{
+    const unsigned long long mine = (exist & (left >= 64 ? ~0ull : (1ull << max(left, 0)) - 1)) >> (4 * g);
+    unsigned part[2] = {(unsigned)mine, (unsigned)(mine >> 32)};
+    asm volatile("" : "+v"(part[0]), "+v"(part[1]));
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (!((part[j >> 1] >> (16 * (j & 1) + r)) & 1))
+                s[j][r] = -INFINITY;
+}
+
 /* workgroup `id` of a CACHED_TILES launch over half tensors, tiles of 64 QR rows. DHC: columns computed with, at least dh (rows of 80
    or 96 columns stand in LDS as rows of 128) */
 template <int DHM, int DHC, int QR>
@@ -220,16 +237,8 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
         const bool cut = exist != ~0ull || key0 + KB > seenMin;
 #pragma unroll
         for (int q = 0; q < QR; q++) {
-            if (cut) {
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int at = 16 * j + 4 * g + r;
-                        if (!((exist >> at) & 1) || key0 + at >= seen[q])
-                            accS[q][j][r] = -INFINITY;
-                    }
-            }
+            if (cut)
+                hide_scores(accS[q], exist, seen[q] - key0, g);
             float mx = accS[q][0][0];
 #pragma unroll
             for (int j = 0; j < NJ; j++)

@@ -149,16 +149,8 @@ __device__ __forceinline__ void attend_tile_f32(const CachedParams & p, int id, 
         const bool cut = exist != ALL || key0 + KB > seenMin;
 #pragma unroll
         for (int q = 0; q < QR; q++) {
-            if (cut) {
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int at = 16 * j + 4 * g + r;
-                        if (!((exist >> at) & 1) || key0 + at >= seen[q])
-                            s[q][j][r] = -INFINITY;
-                    }
-            }
+            if (cut)
+                hide_scores(s[q], exist, seen[q] - key0, g);
             float mx = s[q][0][0];
 #pragma unroll
             for (int j = 0; j < NJ; j++)

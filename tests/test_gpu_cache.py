@@ -181,6 +181,8 @@ TILES = [
     ((8, 70, 64, 64, 8, 88, 16, True, False), 128, False),
     ((8, 70, 64, 64, 8, 128, 16, True, True), 128, False),
     ((8, 1700, 40, 4, 2, 96, 16, True, True), 128, True),
+    ((3, 1100, 1000, 32, 8, 64, 16, True, True), 64, False),                      # more than run at once, long: the longest first
+    ((3, 1100, 1000, 16, 8, 32, 16, False, False), 64, False),
 ]
 
 
