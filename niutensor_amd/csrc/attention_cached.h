@@ -333,7 +333,7 @@ int launch_attention_pairs(const CachedParams & p, bool half, int tile, bool wid
 int launch_attention_tiles(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream);
 int launch_attention_tile_rows(const CachedParams & p, int tile, int blocks, hipStream_t stream);
 constexpr int CACHED_TILE_KEYS = 64;
-/* both launches of a shared prefix in one: `pre` over it in tiles of `tile` rows (64 or 128 half, 16 or 32 float), `own` over each
+/* both launches of a shared prefix in one: `pre` over it in tiles of `tile` rows (64 or 128 half, 16, 32 or 64 float), `own` over each
    sequence's own keys, 16 qr rows */
 int launch_attention_prefix(const CachedParams & pre, const CachedParams & own, bool half, int tile, int qr, int preBlocks,
                             int ownBlocks, hipStream_t stream);

@@ -8,19 +8,20 @@
  */
 #include "attention_cached_rows.h"
 #include "attention_cached_tiles.h"
+#include "attention_cached_tiles_f32.h"
 
 namespace ntsamd {
 
 namespace {
 
-/* TILE: rows of a tile of the prefix (16 and 32 float, 64 and 128 half); QR: blocks of 16 rows of a sequence's own */
+/* TILE: rows of a tile of the prefix (16, 32 and 64 float, 64 and 128 half); QR: blocks of 16 rows of a sequence's own */
 template <typename T, int DHM, int TILE, int QR>
 __global__ void __launch_bounds__(256, 2)
 attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preBlocks, int ownBlocks)
 {
     __shared__ union Shared {
         CachedShared<DHM, 4> rows;
-        CachedTilesShared<half_t, DHM == 96 ? 32 : DHM> tiles;      /* half only, which has no 96 */
+        CachedTilesShared<T, DHM == 96 ? 128 : DHM> tiles;
         __device__ Shared() {}
     } sh;
     const int id = (int)blockIdx.x, both = 2 * (min(preBlocks, ownBlocks) & ~7);
@@ -37,8 +38,10 @@ attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preB
             at -= preBlocks - both / 2;
     }
     if (first) {
-        if constexpr (TILE > 32)
+        if constexpr (sizeof(T) == 2)
             attend_tile<DHM, DHM, TILE / 64>(pre, at, sh.tiles);
+        else if constexpr (TILE == 64)
+            attend_tile_f32<DHM == 96 ? 128 : DHM, DHM>(pre, at, sh.tiles);
         else
             attend_tile_rows<T, DHM, TILE / 16>(pre, at, sh.rows);
     }
@@ -65,6 +68,8 @@ int launch_dhm(const CachedParams & pre, const CachedParams & own, bool half, in
         if (half)
             return tile <= 64 ? launch_tile<half_t, DHM, 64>(pre, own, qr, preBlocks, ownBlocks, stream)
                               : launch_tile<half_t, DHM, 128>(pre, own, qr, preBlocks, ownBlocks, stream);
+    if (tile > 32)
+        return launch_tile<float, DHM, 64>(pre, own, qr, preBlocks, ownBlocks, stream);
     return tile <= 16 ? launch_tile<float, DHM, 16>(pre, own, qr, preBlocks, ownBlocks, stream)
                       : launch_tile<float, DHM, 32>(pre, own, qr, preBlocks, ownBlocks, stream);
 }

@@ -1183,22 +1183,26 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 pre.mode = CACHED_TILES;
                 pre.first = 0;
                 pre.prefix = prefix;
-                pre.rows = half ? (all <= 64 ? 64 : 128) : (all <= 16 ? 16 : 32);
-                pre.tiles = (int)((all + pre.rows - 1) / pre.rows);
-                /* pieces of its keys by the estimate for tiles, which is without the sequences' own keys: one workgroup to a CU
-                   beside many of theirs, two beside few */
-                const long long slots = (long long)pre.tiles * kv;
+                /* rows of its tiles and pieces of its keys by the estimate for tiles, which is without the sequences' own keys: one
+                   workgroup to a CU beside many of theirs, two beside few */
                 long long pieces = 1;
                 double best = -1.0;
-                for (int of = 1; of <= 64; of += of < 4 ? 1 : of / 4) {
-                    if (of > 1 && (slots * of > (pairs >= cus / 2 ? 1 : 2) * cus || CACHED_TILE_KEYS * of > prefix || slots * pre.rows * of > (cut ? room / 2 : room - pairs * rows)))
-                        break;
-                    const double t = cached_tiles_cost(half, dh, pre.rows, slots, prefix, of, slots * pre.rows, 0.0);
-                    if (best < 0.0 || t < best) {
-                        best = t;
-                        pieces = of;
+                for (int rowsOf = half ? 64 : 16; rowsOf <= (half ? 128 : 64); rowsOf *= 2) {
+                    const long long slots = (all + rowsOf - 1) / rowsOf * kv;
+                    for (int of = 1; of <= 64; of += of < 4 ? 1 : of / 4) {
+                        if (of > 1 && (slots * of > (pairs >= cus / 2 ? 1 : 2) * cus || CACHED_TILE_KEYS * of > prefix ||
+                                       slots * rowsOf * of > (cut ? room / 2 : room - pairs * rows)))
+                            break;
+                        const double t = cached_tiles_cost(half, dh, rowsOf, slots, prefix, of, slots * rowsOf, 0.0);
+                        if (best < 0.0 || t < best) {
+                            best = t;
+                            pieces = of;
+                            pre.rows = rowsOf;
+                        }
                     }
                 }
+                pre.tiles = (int)((all + pre.rows - 1) / pre.rows);
+                const long long slots = (long long)pre.tiles * kv;
                 pre.groups = (int)pieces;
                 preBlocks = slots * pre.groups;
                 used = preBlocks * pre.rows;

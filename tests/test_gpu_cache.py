@@ -323,6 +323,45 @@ def test_prefix(gpu, lens, new, heads, kv, dh, page, half, causal, prefix, layou
     assert (out == first).all()
 
 
+PREFIX_TILES = [
+    # sequences, new tokens, prefix, heads, kv, dh, half: the tiles' rows
+    ((60, 4, 1024, 4, 4, 32, False), 32),
+    ((20, 4, 1024, 16, 2, 84, False), 32),
+    ((20, 4, 512, 32, 8, 32, False), 64),
+    ((20, 4, 1024, 32, 4, 64, False), 64),
+    ((20, 4, 1024, 64, 8, 96, False), 64),
+    ((20, 4, 1024, 64, 8, 128, False), 64),
+    ((20, 4, 1024, 64, 8, 32, True), 128),
+    ((60, 4, 1024, 32, 4, 64, True), 128),
+    ((20, 4, 1024, 64, 8, 88, True), 128),
+    ((60, 4, 1024, 32, 4, 128, True), 128),
+]
+
+
+@pytest.mark.parametrize("sizes,rows", PREFIX_TILES)
+def test_every_kind_of_tile_of_the_prefix(gpu, sizes, rows):
+    n, new, prefix, heads, kv, dh, half = sizes
+    p = Problem([prefix + 40 - 2 * i if i != 3 else 300 for i in range(n)], [new - i % 3 for i in range(n)], heads, kv, dh, 32, half, 24,
+                prefix=prefix, pad_tokens=2)
+    cache, batch, q, out = p.place(nt)
+    want, tol = p.attention(True)
+    nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    assert "x%d pieces=" % rows in nt.last_plan() and "prefix" in nt.last_plan(), nt.last_plan()
+    assert_within(out, want, tol, nt.last_plan())
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("prefix", [100, 1000, 1015])
+def test_prefix_of_any_length(gpu, half, prefix):
+    """A prefix need not end with a page: the page in which it ends is read through the first row for its part of it."""
+    p = Problem([1030, 1100, 1015], [1, 1, 1], 4, 2, 64, 16, half, 25, prefix=1008, uniform=True)
+    p.table[1:, 63] = p.table[0, 63]                                               # the rest of that page holds positions of all three
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    assert_within(out, want, tol, nt.last_plan())
+
+
 def test_prefix_is_read_through_the_first_row_of_the_table(gpu):
     """The other sequences' entries for the prefix are not looked at."""
     p = Problem([140, 150, 160], [1, 1, 1], 4, 2, 64, 16, True, 22, prefix=128, uniform=True)
