@@ -153,11 +153,10 @@ __device__ __forceinline__ void sort_sequences(const CachedParams & p, CachedSca
 {
     const int lane = threadIdx.x & 63;
     const int length = lane < p.seqs ? cache_sequence(p.c, p.seq0 + lane).length : 0;
+    const int key = min(length, 0x1ffffff) << 6 | lane;             /* no two alike */
     int rank = 0;
-    for (int i = 0; i < p.seqs; i++) {
-        const int other = __builtin_amdgcn_readlane(length, i);
-        rank += other < length || (other == length && i < lane) ? 1 : 0;
-    }
+    for (int i = 0; i < p.seqs; i++)
+        rank += __builtin_amdgcn_readlane(key, i) < key ? 1 : 0;
     if (threadIdx.x < p.seqs)
         sh.order[rank] = lane;
     __syncthreads();

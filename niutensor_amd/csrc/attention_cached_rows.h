@@ -362,7 +362,11 @@ __device__ __forceinline__ Segment pair_segment(const CachedParams & p, CachedSc
     else {
         i = id / p.c.kvHeads;
         head = id - i * p.c.kvHeads;
-        slot = p.acc ? id : -1;
+        if (p.sorted) {
+            sort_sequences(p, sh);
+            i = sh.order[p.seqs - 1 - i];
+        }
+        slot = p.acc ? i * p.c.kvHeads + head : -1;
     }
     Segment sg;
     sg.seq = p.seq0 + i;

@@ -351,6 +351,20 @@ def test_every_kind_of_tile_of_the_prefix(gpu, sizes, rows):
 
 
 @pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("n,prefix", [(62, 512), (64, 512), (64, 1024)])
+def test_prefix_of_uneven_sequences(gpu, half, n, prefix):
+    """62 do not fill the part and are cut into pieces; 64 are left whole. Behind 1024 positions they are more workgroups than run at
+    once: the longest sequences come first, whichever place they have in the batch."""
+    p = Problem([prefix + i * 37 % 300 for i in range(n)], [1] * n, 8, 8, 32, 16, half, 26, prefix=prefix, uniform=True)
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    if prefix == 1024:
+        assert "prefix" in nt.last_plan() and "whole=512" in nt.last_plan(), nt.last_plan()
+    assert_within(out, want, tol, nt.last_plan())
+
+
+@pytest.mark.parametrize("half", [True, False])
 @pytest.mark.parametrize("prefix", [100, 1000, 1015])
 def test_prefix_of_any_length(gpu, half, prefix):
     """A prefix need not end with a page: the page in which it ends is read through the first row for its part of it."""
