@@ -95,7 +95,7 @@ int ntsamd_cache_append(int devID, void * stream, const ntsamd_cache * cache, co
  * never used, whatever its bits. Inside a sequence, a value that is not finite reaches every token that sees it,
  * and may reach, as NaN, tokens of the same sequence and call that stand before it.
  *   strides[0], strides[1]: token and head of q; strides[2], strides[3]: of out. q and out are 16-byte aligned, their strides
- *   multiples of 4 (float) or 8 (half) elements. Data types, rounding and accumulation as in ntsamd_attention: half products with fp32
+ *   multiples of 4 (float) or 8 (half) elements; out overlaps nothing else. Data types, rounding and accumulation as in ntsamd_attention: half products with fp32
  *   accumulation, softmax in fp32, probabilities rounded to half before the second product.
  * Long sequences are cut into pieces whose partial results meet in the stream's workspace (ntsamd_gemm.h) and are
  * added up by a second kernel, always in the same order; without a workspace they run in one piece.

@@ -290,6 +290,61 @@ def test_pool_beyond_four_gigabytes(gpu):
     assert_within(out, want[[149, 249]], tol[[149, 249]], "large pool, one token")
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new", [1, 20])
+def test_pages_of_one_position_and_no_pages_at_all(gpu, half, new):
+    import torch
+    p = Problem([70, 20, 133], [new] * 3, 4, 2, 64, 1, half, 61, uniform=True)
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_cached(cache, batch, q, out, p.scale)
+    assert_within(out, want, tol, nt.last_plan())
+    none = nt.CacheBatch(p.lengths_d, p.table_d[:, :0].contiguous(), tokens=p.tokens, max_new=new)
+    for prefix in (None, 64):
+        out.fill_(77.0)
+        if prefix is None:
+            nt.attention_cached(cache, none, q, out, p.scale)
+        else:
+            nt.attention_prefix(cache, none, q, out, p.scale, prefix)
+        assert (out == 0).all()                                                    # tokens that see nothing
+    before = p.kd.clone()
+    k = torch.ones((p.tokens, 2, 64), dtype=q.dtype, device=gpu)
+    nt.cache_append(cache, none, k, k, q=q, q_out=out.fill_(77.0))
+    assert torch.equal(torch.nan_to_num(p.kd), torch.nan_to_num(before)) and (out == 77).all()
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,prefix", [(1, None), (12, None), (1, 512)])
+def test_more_rows_than_a_uniform_batch_has(gpu, half, new, prefix):
+    p = Problem([600, 545, 570], [new] * 3, 8, 2, 64, 16, half, 62, prefix=prefix or 0, uniform=True, pad_tokens=5)
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    if prefix:
+        nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    else:
+        nt.attention_cached(cache, batch, q, out, p.scale)
+    assert_within(out, want, tol, nt.last_plan())
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,prefix", [(1, None), (40, None), (1, 512)])
+def test_lengths_and_starts_are_held_to_their_bounds(gpu, half, new, prefix):
+    """A negative length is none, one beyond max_length is max_length, starts outside the rows end with them: every kernel holds what it
+    reads to the bounds it was given, so that the other sequences come out right, and nothing else is touched."""
+    import torch
+    p = Problem([560, 550, 700, 640], [new] * 4, 8, 2, 64, 16, half, 63, prefix=prefix or 0, max_length=700, slack=0)
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    p.lengths_d.copy_(torch.tensor([560, -5, 2 ** 31 - 1, 640], dtype=torch.int32))
+    p.starts_d[0], p.starts_d[4] = -7, 2 ** 30
+    want[new:2 * new], tol[new:2 * new] = 0.0, 0.0
+    if prefix:
+        nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    else:
+        nt.attention_cached(cache, batch, q, out, p.scale)
+    assert_within(out, want, tol, nt.last_plan())
+
+
 # ---- sequences with a common beginning ----------------------------------------------------------------------------
 
 PREFIX = [
