@@ -45,10 +45,10 @@ template <typename T, int DHM> struct CachedTilesShared {
 };
 
 /* global memory -> LDS, 16 bytes per lane: lane l's data lands at lds + 16 l (the same for the whole wave). Counted by vmcnt, which
-   the caller waits for: the compiler does not see a load */
+   the caller waits for: the compiler does not see a load. An instruction that reads M0 for LDS must not follow its write at once. */
 __device__ __forceinline__ void lds_from_global16(unsigned lds, long long address)
 {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(lds), "v"(address)
                  : "memory");
