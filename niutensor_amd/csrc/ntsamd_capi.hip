@@ -1030,13 +1030,13 @@ int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, Ca
 
 /* Run time of a cached attention in tiles, in microseconds, fitted to graph-replayed calls on 8 to 2048 workgroups, heads of 32, 64,
    96 and 128, 1024 to 4096 keys, and to calls of uneven lengths. A workgroup alone on its CU takes `alone` for every 64 keys; 256 CUs
-   take `busy` for 64 keys of every 256 workgroups where more of them share a CU. With more workgroups than CUs it is half of that (of
-   the lengths, about half is there) and most of the longest one's own time. Tiles of fewer rows read the keys more often and take
+   take `busy` for 64 keys of every 256 workgroups where more of them share a CU. With more workgroups than CUs it is the part of that
+   which is `there` (about half, where many sequences have lengths up to the bound) and most of the longest one's own time. Tiles of fewer rows read the keys more often and take
    fewer rows per MFMA's keys, but there are more of them, and shorter ones. Keys cut into pieces: as many workgroups for fewer keys, a
    join (`join` us), and their partial rows written and read (about 6 TB/s, most of it behind the multiplications).
    Float, 13 pieces of text of up to 784 tokens behind up to 3282, 8 heads of 128 on one key head, tiles of 16, 32, 64 rows: 774,
    661, 719 us; 45 of 567 of 829, 32 on 8 of 64: 955, 879, 731; 36 of 339 of 2425, 16 on 4 of 96, half, 64 and 128: 176, 134. */
-double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long long keys, int pieces, long long rows, double join)
+double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long long keys, double there, int pieces, long long rows, double join)
 {
     static const double alone[5][4] = {{0.87, 1.17, 1.50, 1.75}, {1.27, 1.79, 2.34, 2.80}, {1.72, 2.71, 4.48, 5.43},
                                        {0.76, 0.96, 1.34, 1.40}, {1.07, 1.28, 1.65, 1.85}};
@@ -1044,7 +1044,7 @@ double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long
                                       {0.38, 0.53, 0.85, 0.90}, {0.63, 0.88, 1.15, 1.25}};
     const int kind = half ? (tile == 64 ? 3 : 4) : (tile == 16 ? 0 : (tile == 32 ? 1 : 2));
     const int width = dh <= 32 ? 0 : (dh <= 64 ? 1 : (dh <= 96 ? 2 : 3));
-    const double a = alone[kind][width], load = (double)workgroups * pieces / 256.0, b = 0.5 * busy[kind][width] * load + 0.8 * a;
+    const double a = alone[kind][width], load = (double)workgroups * pieces / 256.0, b = there * busy[kind][width] * load + 0.8 * a;
     const double blocks = (double)((keys + 63) / 64 + pieces - 1) / pieces;
     return blocks * (load <= 1.0 || a > b ? a : b) + (pieces > 1 ? join + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 6.0e6 : 0.0);
 }
@@ -1104,7 +1104,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 if (cut > 1 && (!mayHold || of * kv * cut > 4 * cus || 2 * CACHED_TILE_KEYS * cut > p.c.maxLength ||
                                 of * kv * tile * cut * slotRow > (long long)SPLIT_WORK_BYTES))
                     break;
-                const double t = cached_tiles_cost(half, dh, tile, of * kv, p.c.maxLength, cut, of * kv * tile, 4.0);
+                const double t = cached_tiles_cost(half, dh, tile, of * kv, p.c.maxLength, n > 1 ? 0.5 : 0.9, cut, of * kv * tile, 4.0);
                 if (best < 0.0 || t < best) {
                     best = t;
                     tiles = of;
@@ -1193,7 +1193,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                         if (of > 1 && (slots * of > (pairs >= cus / 2 ? 1 : 2) * cus || CACHED_TILE_KEYS * of > prefix ||
                                        slots * rowsOf * of > (cut ? room / 2 : room - pairs * rows)))
                             break;
-                        const double t = cached_tiles_cost(half, dh, rowsOf, slots, prefix, of, slots * rowsOf, 0.0);
+                        const double t = cached_tiles_cost(half, dh, rowsOf, slots, prefix, 0.9, of, slots * rowsOf, 0.0);
                         if (best < 0.0 || t < best) {
                             best = t;
                             pieces = of;
