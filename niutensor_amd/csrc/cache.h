@@ -77,8 +77,7 @@ struct AppendParams {
     long long kT, kH, vT, vH, qT, qH, oT, oH;
     const float * rotation;             /* NULL: nothing is turned */
     int positions, rotated, pairing;
-    int items;                          /* filled in by the launcher: pieces of work per token, waves per token */
-    int waves;
+    int items, perWave, waves;          /* filled in by the launcher: pieces of work per token, of them per wave, waves per token */
 };
 
 struct CachedParams {

@@ -6,14 +6,14 @@
  *
  * Bound by memory: every new row is read once and written once, and one row of the rotation per token serves all
  * heads. A token's work is cut into items: 16 bytes of a row that is copied, twice 16 bytes where column j is turned
- * together with column j + rotated / 2 (both pieces by one lane, so that q may be turned in place). A wave takes up
- * to 256 items of one token: it finds the token's sequence once, by counting the starts that are not behind the token,
+ * together with column j + rotated / 2 (both pieces by one lane, so that q may be turned in place). A wave takes 64, 128 or
+ * 256 items of one token: it finds the token's sequence once, by counting the starts that are not behind the token,
  * 64 to a load (a binary search would chain a load per step in front of the two it cannot do without: the page number
  * and the row itself).
  * Rows that are not 16-byte aligned and numbers of turned columns that are no whole 16-byte pieces take items of one
  * column or pair instead.
- * 8 prompts of 513 to 2048 tokens, 32 heads on 8 of 128 columns, half: 47 us, 5.0 TB/s read and written; one token: 3.8 us, a launch and
- * the three loads; 64 sequences of one token: 4.6.
+ * 8 prompts of 513 to 2048 tokens, 32 heads on 8 of 128 columns, half: 46 us, 5.1 TB/s read and written; one token: 3.5 us, a launch and
+ * the three loads; 64 sequences of one token: 3.5.
  */
 #include "gemm_common.h"
 #include "gemm_f16.h"       /* half_t */
@@ -22,8 +22,6 @@
 namespace ntsamd {
 
 namespace {
-
-constexpr int ITEMS_PER_WAVE = 256;
 
 /* N consecutive columns as floats */
 template <typename T, int N> struct Columns {
@@ -149,8 +147,8 @@ cache_append_kernel(const AppendParams p)
     const int copied = (c.dh - (p.rotation ? p.rotated : 0)) / N;
     const int perRow = turned + copied;                 /* items of a row of k or q; of v: dh / N */
     const int kItems = c.kvHeads * perRow, vItems = c.kvHeads * (c.dh / N);
-    const int end = min(p.items, (part + 1) * ITEMS_PER_WAVE);
-    for (int i = part * ITEMS_PER_WAVE + lane; i < end; i += 64) {
+    const int end = min(p.items, (part + 1) * p.perWave);
+    for (int i = part * p.perWave + lane; i < end; i += 64) {
         if (i < kItems) {
             const int h = i / perRow;
             if (stored)
@@ -176,7 +174,13 @@ int launch(AppendParams p, hipStream_t stream)
 {
     const int turned = turned_pieces<N>(p), perRow = turned + (p.c.dh - (p.rotation ? p.rotated : 0)) / N;
     p.items = p.c.kvHeads * (perRow + p.c.dh / N) + (p.q ? p.heads * perRow : 0);
-    p.waves = (p.items + ITEMS_PER_WAVE - 1) / ITEMS_PER_WAVE;
+    /* A lane's items follow one another, each a load and a store that wait for memory: one each where the waves run at once (64 sequences
+       of one token, 448 waves: 3.5 us; 4.6 with four). Beyond, what a wave does first counts, its look at the starts above all: two each
+       (1 to 499 tokens of 7 sequences, float: 9.3, 7.7, 8.4 us with one, two and four; 8 prompts 48.5, 45.7, 47.5), four with more
+       than 64 sequences (87 of up to 108 tokens: 13.9, 11.8, 9.9). */
+    const int looks = p.c.starts ? p.c.sequences / 64 + 1 : 1;
+    p.perWave = (long long)p.c.tokens * ((p.items + 63) / 64) * looks <= 1024 ? 64 : (looks == 1 ? 128 : 256);
+    p.waves = (p.items + p.perWave - 1) / p.perWave;
     const long long blocks = ((long long)p.c.tokens * p.waves + 3) / 4;
     if (blocks > 0x1fffffffLL)                          /* the kernel counts waves in 32 bits */
         return (int)hipErrorInvalidValue;

@@ -30,6 +30,8 @@ APPEND = [
     ([9, 30], [9, 21], 2, 1, 20, 5, False, 6, True, "heads", False),
     ([200] * 130, [1] * 130, 2, 2, 32, 32, False, 0, False, "rows", False),        # more starts than a wave has lanes
     ([7, 8], [3, 3], 4, 2, 128, 4, True, None, False, "heads", True),              # no rotation at all
+    ([30 + i % 5 for i in range(70)], [20 - i % 7 for i in range(70)], 8, 4, 64, 16, True, 64, False, "rows", False),   # many of both
+    ([300, 310], [290, 300], 8, 4, 128, 16, False, 128, False, "heads", False),
 ]
 
 
