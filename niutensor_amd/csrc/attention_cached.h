@@ -8,7 +8,7 @@
 namespace ntsamd {
 
 struct CachedScan {
-    long long sums[4];
+    long long sums[8];
     long long before;
     int found;
     int order[64];
@@ -21,18 +21,18 @@ __device__ __forceinline__ int units_of(const CachedParams & p, const CacheSeque
     return s.fresh > 0 ? max((max(s.length - p.first, 0) + UK - 1) / UK, 1) : 0;
 }
 
-/* Sums over the sequences of a launch, weight(i) each: every thread of the 256 takes a run of sequences. */
+/* Sums over the sequences of a launch, weight(i) each: every thread of the 64 NW takes a run of sequences. */
 struct SequenceScan {
     long long before, sum, total;       /* of the sequences before this thread's, of this thread's, of all */
     int from, to;                       /* this thread's sequences */
 };
 
-template <typename W>
+template <int NW = 4, typename W>
 __device__ __forceinline__ SequenceScan scan_sequences(int count, CachedScan & sh, W weight)
 {
     SequenceScan r;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int run = (count + 255) / 256;
+    const int run = (count + 64 * NW - 1) / (64 * NW);
     r.from = min(tid * run, count);
     r.to = min(r.from + run, count);
     r.sum = 0;
@@ -51,7 +51,7 @@ __device__ __forceinline__ SequenceScan scan_sequences(int count, CachedScan & s
     r.before = upTo - r.sum;
     r.total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < NW; w++) {
         if (w < wave)
             r.before += sh.sums[w];
         r.total += sh.sums[w];
@@ -162,8 +162,8 @@ __device__ __forceinline__ void sort_sequences(const CachedParams & p, CachedSca
     __syncthreads();
 }
 
-/* CACHED_TILES: the segment of workgroup `id`, tiles of TR rows, units of UK keys; without rows where it has none */
-template <int TR, int UK>
+/* CACHED_TILES: the segment of workgroup `id` of NW waves, tiles of TR rows, units of UK keys; without rows where it has none */
+template <int TR, int UK, int NW = 4>
 __device__ __forceinline__ Segment tile_segment(const CachedParams & p, CachedScan & sh, int id)
 {
     /* the last tiles of a sequence see the most keys: first. Where there are more workgroups than run at once, those of the longest
@@ -182,7 +182,7 @@ __device__ __forceinline__ Segment tile_segment(const CachedParams & p, CachedSc
             sort_sequences(p, sh);
         const auto sequence = [&](int n) { return p.seq0 + (p.sorted ? sh.order[n] : n); };
         const auto tiles = [&](int n) { return (long long)((cache_sequence(p.c, sequence(n)).fresh * p.per + TR - 1) / TR); };
-        const SequenceScan scan = scan_sequences(p.seqs, sh, tiles);
+        const SequenceScan scan = scan_sequences<NW>(p.seqs, sh, tiles);
         long long before = 0;
         const int i = find_sequence(scan, tile, before, sh, tiles);
         seq = sequence(max(i, 0));
@@ -328,9 +328,10 @@ __device__ __forceinline__ V load_global(long long address)
 /* CACHED_WHOLE, CACHED_PIECES: `tile` (16 or 32) rows to a pair at most. wide: CACHED_WHOLE without partial results, up to 16 rows,
    as many waves to a workgroup as a CU runs */
 int launch_attention_pairs(const CachedParams & p, bool half, int tile, bool wide, int blocks, hipStream_t stream);
-/* CACHED_TILES: tiles of 64 or 128 (half) rows; float tiles of 16 or 32 */
+/* CACHED_TILES: tiles of 64 or 128 (half) rows; tiles of 16 (half, float) or 32 (float) rows whose
+   waves share out the keys */
 int launch_attention_tiles(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream);
-int launch_attention_tile_rows(const CachedParams & p, int tile, int blocks, hipStream_t stream);
+int launch_attention_tile_rows(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream);
 constexpr int CACHED_TILE_KEYS = 64;
 /* both launches of a shared prefix in one: `pre` over it in tiles of `tile` rows (64 or 128 half, 16, 32 or 64 float), `own` over each
    sequence's own keys, 16 qr rows */

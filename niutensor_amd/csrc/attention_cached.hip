@@ -19,13 +19,14 @@ attention_cached_kernel(const CachedParams p)
     attend_pair<T, DHM, QR, NW>(p, (int)blockIdx.x, sh);
 }
 
-/* CACHED_TILES, float tiles of 16 or 32 rows (more rows, and half: attention_cached_tiles.hip) */
-template <int DHM, int QR>
-__global__ void __launch_bounds__(256, 2)
+/* CACHED_TILES, tiles of 16 or 32 rows (more rows: attention_cached_tiles.hip). NW: 4 waves; in half 8, for calls whose workgroups all
+   run at once (float keeps the matrix unit busy with 4: 16.4 us with 4, 14.2 with 8 for 1024 keys of 32 columns, 31 and 35 of 128) */
+template <typename T, int DHM, int QR, int NW>
+__global__ void __launch_bounds__(64 * NW, NW == 8 && DHM <= 64 ? 4 : 2)
 attention_cached_tile_kernel(const CachedParams p)
 {
-    __shared__ CachedShared<DHM, 4> sh;
-    attend_tile_rows<float, DHM, QR>(p, (int)blockIdx.x, sh);
+    __shared__ CachedShared<DHM, NW> sh;
+    attend_tile_rows<T, DHM, QR, NW>(p, (int)blockIdx.x, sh);
 }
 
 template <typename T, int DHM>
@@ -54,14 +55,29 @@ int launch_type(const CachedParams & p, int tile, bool wide, int blocks, hipStre
     return launch_pairs<T, 128>(p, tile, wide, blocks, stream);
 }
 
-template <int DHM>
+template <typename T, int DHM>
 int launch_tile(const CachedParams & p, int tile, int blocks, hipStream_t stream)
 {
-    if (tile == 16)
-        hipLaunchKernelGGL((attention_cached_tile_kernel<DHM, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    if constexpr (sizeof(T) == 2)
+        hipLaunchKernelGGL((attention_cached_tile_kernel<T, DHM, 1, 8>), dim3((unsigned)blocks), dim3(512), 0, stream, p);
+    else if (tile == 16)
+        hipLaunchKernelGGL((attention_cached_tile_kernel<T, DHM, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     else
-        hipLaunchKernelGGL((attention_cached_tile_kernel<DHM, 2>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((attention_cached_tile_kernel<T, DHM, 2, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     return (int)hipGetLastError();
+}
+
+template <typename T>
+int launch_tile_type(const CachedParams & p, int tile, int blocks, hipStream_t stream)
+{
+    if (p.c.dh <= 32)
+        return launch_tile<T, 32>(p, tile, blocks, stream);
+    if (p.c.dh <= 64)
+        return launch_tile<T, 64>(p, tile, blocks, stream);
+    if constexpr (sizeof(T) == 4)
+        if (p.c.dh <= 96)
+            return launch_tile<T, 96>(p, tile, blocks, stream);
+    return launch_tile<T, 128>(p, tile, blocks, stream);
 }
 
 }  // namespace
@@ -71,15 +87,9 @@ int launch_attention_pairs(const CachedParams & p, bool half, int tile, bool wid
     return half ? launch_type<half_t>(p, tile, wide, blocks, stream) : launch_type<float>(p, tile, wide, blocks, stream);
 }
 
-int launch_attention_tile_rows(const CachedParams & p, int tile, int blocks, hipStream_t stream)
+int launch_attention_tile_rows(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream)
 {
-    if (p.c.dh <= 32)
-        return launch_tile<32>(p, tile, blocks, stream);
-    if (p.c.dh <= 64)
-        return launch_tile<64>(p, tile, blocks, stream);
-    if (p.c.dh <= 96)
-        return launch_tile<96>(p, tile, blocks, stream);
-    return launch_tile<128>(p, tile, blocks, stream);
+    return half ? launch_tile_type<half_t>(p, tile, blocks, stream) : launch_tile_type<float>(p, tile, blocks, stream);
 }
 
 }  // namespace ntsamd

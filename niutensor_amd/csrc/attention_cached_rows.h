@@ -384,13 +384,13 @@ __device__ __forceinline__ Segment pair_segment(const CachedParams & p, CachedSc
     return sg;
 }
 
-/* workgroup `id` of a CACHED_TILES launch, tiles of 16 QR rows */
-template <typename T, int DHM, int QR>
-__device__ __forceinline__ void attend_tile_rows(const CachedParams & p, int id, CachedShared<DHM, 4> & sh)
+/* workgroup `id` of a CACHED_TILES launch, tiles of 16 QR rows, NW waves */
+template <typename T, int DHM, int QR, int NW>
+__device__ __forceinline__ void attend_tile_rows(const CachedParams & p, int id, CachedShared<DHM, NW> & sh)
 {
-    const Segment sg = uniform(tile_segment<16 * QR, Unit<T, DHM>::UK>(p, sh.scan, id));
+    const Segment sg = uniform(tile_segment<16 * QR, Unit<T, DHM>::UK, NW>(p, sh.scan, id));
     if (sg.rows > 0)
-        attend<T, DHM, QR, 4>(p, sg, sh);
+        attend<T, DHM, QR, NW>(p, sg, sh);
 }
 
 /* workgroup `id` of a CACHED_WHOLE or CACHED_PIECES launch, NW waves (more than 4: CACHED_WHOLE only, scans take 256 threads) */

@@ -45,7 +45,7 @@ attention_prefix_kernel(const CachedParams pre, const CachedParams own, int preB
         else if constexpr (TILE == 64)
             attend_tile_f32<DHM == 96 ? 128 : DHM, DHM>(pre, at, sh.tiles);
         else
-            attend_tile_rows<T, DHM, TILE / 16>(pre, at, sh.rows);
+            attend_tile_rows<T, DHM, TILE / 16, 4>(pre, at, sh.rows);
     }
     else
         attend_pair<T, DHM, QR, 4>(own, at, sh.rows);

@@ -1036,17 +1036,23 @@ int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, Ca
    join (`join` us), and their partial rows written and read (about 6 TB/s, most of it behind the multiplications).
    Float, 13 pieces of text of up to 784 tokens behind up to 3282, 8 heads of 128 on one key head, tiles of 16, 32, 64 rows: 774,
    661, 719 us; 45 of 567 of 829, 32 on 8 of 64: 955, 879, 731; 36 of 339 of 2425, 16 on 4 of 96, half, 64 and 128: 176, 134. */
-double cached_tiles_cost(bool half, int dh, int tile, long long workgroups, long long keys, double there, int pieces, long long rows, double join)
+struct TileKind {
+    int rows, threads;                  /* of a tile, of its workgroup */
+    double alone[4], busy[4];           /* heads of up to 32, 64, 96, 128 columns */
+};
+const TileKind g_tileKinds[2][3] = {{{16, 256, {0.87, 1.17, 1.50, 1.75}, {0.50, 0.85, 1.46, 1.65}},
+                                     {32, 256, {1.27, 1.79, 2.34, 2.80}, {0.85, 1.45, 2.36, 2.65}},
+                                     {64, 256, {1.72, 2.71, 4.48, 5.43}, {1.39, 2.39, 3.69, 4.60}}},
+                                    {{16, 512, {0.28, 0.42, 0.66, 0.66}, {0.34, 0.46, 0.95, 0.95}},
+                                     {64, 256, {0.76, 0.96, 1.34, 1.40}, {0.38, 0.53, 0.85, 0.90}},
+                                     {128, 256, {1.07, 1.28, 1.65, 1.85}, {0.63, 0.88, 1.15, 1.25}}}};
+
+double cached_tiles_cost(const TileKind & kind, int dh, long long workgroups, long long keys, double there, int pieces, double join)
 {
-    static const double alone[5][4] = {{0.87, 1.17, 1.50, 1.75}, {1.27, 1.79, 2.34, 2.80}, {1.72, 2.71, 4.48, 5.43},
-                                       {0.76, 0.96, 1.34, 1.40}, {1.07, 1.28, 1.65, 1.85}};
-    static const double busy[5][4] = {{0.50, 0.85, 1.46, 1.65}, {0.85, 1.45, 2.36, 2.65}, {1.39, 2.39, 3.69, 4.60},
-                                      {0.38, 0.53, 0.85, 0.90}, {0.63, 0.88, 1.15, 1.25}};
-    const int kind = half ? (tile == 64 ? 3 : 4) : (tile == 16 ? 0 : (tile == 32 ? 1 : 2));
     const int width = dh <= 32 ? 0 : (dh <= 64 ? 1 : (dh <= 96 ? 2 : 3));
-    const double a = alone[kind][width], load = (double)workgroups * pieces / 256.0, b = there * busy[kind][width] * load + 0.8 * a;
+    const double a = kind.alone[width], load = (double)workgroups * pieces / 256.0, b = there * kind.busy[width] * load + 0.8 * a;
     const double blocks = (double)((keys + 63) / 64 + pieces - 1) / pieces;
-    return blocks * (load <= 1.0 || a > b ? a : b) + (pieces > 1 ? join + 2.0 * (double)rows * pieces * (dh + 2) * 4 / 6.0e6 : 0.0);
+    return blocks * (load <= 1.0 || a > b ? a : b) + (pieces > 1 ? join + 2.0 * (double)workgroups * kind.rows * pieces * (dh + 2) * 4 / 6.0e6 : 0.0);
 }
 
 /* Whether long keys of few rows are better left whole, a workgroup of as many waves as a CU runs to each pair, than cut into pieces
@@ -1095,7 +1101,8 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         p.mode = CACHED_TILES;
         long long tiles = 0, pieces = 1;
         double best = -1.0;
-        for (int tile = half ? 64 : 16; tile <= (half ? 128 : 64); tile *= 2) {
+        for (const TileKind & kind : g_tileKinds[half ? 1 : 0]) {
+            const int tile = kind.rows;
             const long long perSeq = (rows + tile - 1) / tile;
             long long of = (long long)p.c.tokens * p.per / tile + n;
             if (!p.c.starts || n * perSeq < of)
@@ -1104,7 +1111,12 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 if (cut > 1 && (!mayHold || of * kv * cut > 4 * cus || 2 * CACHED_TILE_KEYS * cut > p.c.maxLength ||
                                 of * kv * tile * cut * slotRow > (long long)SPLIT_WORK_BYTES))
                     break;
-                const double t = cached_tiles_cost(half, dh, tile, of * kv, p.c.maxLength, n > 1 ? 0.5 : 0.9, cut, of * kv * tile, 4.0);
+                /* workgroups of 8 waves, one to a CU (two with narrow heads), start slowly: only as many as run at once (26 pieces of up to
+                   163 tokens, 4 heads of 64, half, 760 workgroups: 18 us, 12.6 in 268 tiles of 64 rows; 2 of up to 35, 16 heads on 8, 56
+                   workgroups: 8.5 and 11.1; 1 of 42, 12 heads on 4 of 32: 5.8 and 7.2) */
+                if (kind.threads > 256 && of * kv * cut > (dh <= 64 ? 2 : 1) * cus)
+                    break;
+                const double t = cached_tiles_cost(kind, dh, of * kv, p.c.maxLength, n > 1 ? 0.5 : 0.9, cut, 4.0);
                 if (best < 0.0 || t < best) {
                     best = t;
                     tiles = of;
@@ -1134,7 +1146,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         if (g_planOnly)
             return NTSAMD_OK;
         rc = p.rows >= 64 ? launch_attention_tiles(p, half, p.rows, (int)(tiles * kv * pieces), stream)
-                          : launch_attention_tile_rows(p, p.rows, (int)(tiles * kv * pieces), stream);
+                          : launch_attention_tile_rows(p, half, p.rows, (int)(tiles * kv * pieces), stream);
         if (rc == 0 && pieces > 1) {
             JoinParams j;
             memset(&j, 0, sizeof(j));
@@ -1187,17 +1199,19 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                    workgroup to a CU beside many of theirs, two beside few */
                 long long pieces = 1;
                 double best = -1.0;
-                for (int rowsOf = half ? 64 : 16; rowsOf <= (half ? 128 : 64); rowsOf *= 2) {
-                    const long long slots = (all + rowsOf - 1) / rowsOf * kv;
+                for (const TileKind & kind : g_tileKinds[half ? 1 : 0]) {
+                    if (kind.threads != 256)
+                        continue;
+                    const long long slots = (all + kind.rows - 1) / kind.rows * kv;
                     for (int of = 1; of <= 64; of += of < 4 ? 1 : of / 4) {
                         if (of > 1 && (slots * of > (pairs >= cus / 2 ? 1 : 2) * cus || CACHED_TILE_KEYS * of > prefix ||
-                                       slots * rowsOf * of > (cut ? room / 2 : room - pairs * rows)))
+                                       slots * kind.rows * of > (cut ? room / 2 : room - pairs * rows)))
                             break;
-                        const double t = cached_tiles_cost(half, dh, rowsOf, slots, prefix, 0.9, of, slots * rowsOf, 0.0);
+                        const double t = cached_tiles_cost(kind, dh, slots, prefix, 0.9, of, 0.0);
                         if (best < 0.0 || t < best) {
                             best = t;
                             pieces = of;
-                            pre.rows = rowsOf;
+                            pre.rows = kind.rows;
                         }
                     }
                 }

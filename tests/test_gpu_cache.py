@@ -182,7 +182,11 @@ TILES = [
     ((8, 70, 64, 64, 8, 64, 20, True, True), 128, False),
     ((8, 70, 64, 64, 8, 88, 16, True, False), 128, False),
     ((8, 70, 64, 64, 8, 128, 16, True, True), 128, False),
-    ((8, 1700, 40, 4, 2, 96, 16, True, True), 128, True),
+    ((8, 1700, 40, 4, 2, 96, 16, True, True), 16, True),
+    ((1, 197, 42, 12, 4, 32, 20, True, True), 16, False),
+    ((2, 568, 35, 16, 8, 64, 16, True, False), 16, False),
+    ((3, 330, 33, 6, 3, 72, 7, True, True), 16, False),
+    ((2, 300, 60, 8, 4, 128, 16, True, True), 16, False),
     ((3, 1100, 1000, 32, 8, 64, 16, True, True), 64, False),                      # more than run at once, long: the longest first
     ((3, 1100, 1000, 16, 8, 32, 16, False, False), 64, False),
 ]
