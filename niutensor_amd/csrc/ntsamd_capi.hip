@@ -1031,9 +1031,10 @@ int check_cache(const ntsamd_cache * cache, const ntsamd_cache_batch * batch, Ca
 /* Run time of a cached attention in tiles, in microseconds, fitted to graph-replayed calls on 8 to 2048 workgroups, heads of 32, 64,
    96 and 128, 1024 to 4096 keys, and to calls of uneven lengths. A workgroup alone on its CU takes `alone` for every 64 keys; 256 CUs
    take `busy` for 64 keys of every 256 workgroups where more of them share a CU. With more workgroups than CUs it is the part of that
-   which is `there` (about half, where many sequences have lengths up to the bound) and most of the longest one's own time. Tiles of fewer rows read the keys more often and take
-   fewer rows per MFMA's keys, but there are more of them, and shorter ones. Keys cut into pieces: as many workgroups for fewer keys, a
-   join (`join` us), and their partial rows written and read (about 6 TB/s, most of it behind the multiplications).
+   which is `there` (about half, where many sequences have lengths up to the bound) and most of the longest one's own time. Tiles of
+   fewer rows read the keys more often and take fewer rows per MFMA's keys, but there are more of them, and shorter ones. Keys cut into
+   pieces: as many workgroups for fewer keys, a join (`join` us), and their partial rows written and read (about 6 TB/s, most of it
+   behind the multiplications).
    Float, 13 pieces of text of up to 784 tokens behind up to 3282, 8 heads of 128 on one key head, tiles of 16, 32, 64 rows: 774,
    661, 719 us; 45 of 567 of 829, 32 on 8 of 64: 955, 879, 731; 36 of 339 of 2425, 16 on 4 of 96, half, 64 and 128: 176, 134. */
 struct TileKind {
@@ -1130,7 +1131,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             if (work.mem == NULL)
                 pieces = 1;
         }
-        if (tiles * kv * pieces > 0x7fffffffLL || (pieces > 1 && tiles * kv * p.rows > 0x7fffffffLL))
+        if (tiles * kv * pieces > 0x7fffffffLL || tiles * p.rows > 0x7fffffffLL || (pieces > 1 && tiles * kv * p.rows > 0x7fffffffLL))
             return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
         p.tiles = (int)tiles;
         p.groups = (int)pieces;

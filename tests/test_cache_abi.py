@@ -144,3 +144,11 @@ def test_plans(planning):
     assert attend(n=1, tokens=1, width=512, prefix=1024) == 0 and "prefix" not in nt.last_plan()
     assert attend(n=8, tokens=8, width=512, prefix=16) == 0 and "prefix" not in nt.last_plan()
     assert append() == 0 and nt.last_plan() == "cache_append_kernel"
+
+
+def test_more_rows_than_a_launch_counts(planning):
+    """500 million tokens of 4 query heads to a key head fit 31 bits, in tiles with one more for every sequence they do not."""
+    big = dict(tokens=500000000, new=1000, width=64, starts=P, heads=8, strides=(512, 64, 512, 64))
+    assert attend(n=1000, **big) == 0
+    assert attend(n=1 << 22, **big) == 1 and "tensor too large" in message()
+    assert attend(n=1000, **dict(big, tokens=600000000)) == 1 and "tensor too large" in message()
