@@ -581,3 +581,84 @@ def test_streams_and_released_workspaces(gpu):
     nt.release_workspaces()
     nt.attention_cached(cache, batch, q, out, p.scale)
     assert_within(out, want, tol, "after a release")
+
+
+def test_two_host_threads_on_one_stream(gpu):
+    """Both threads' calls share the stream's workspace: neither's pieces get between the other's kernels."""
+    import threading
+    import torch
+    problems = [Problem([3000, 100, 2500], [1, 1, 1], 8, 2, 128, 16, True, 71), Problem([2000, 700], [30, 40], 8, 2, 64, 16, False, 72),
+                Problem([1300, 1400, 1290], [1, 1, 1], 8, 2, 64, 16, True, 73, prefix=1280, uniform=True)]
+    jobs = []
+    for p in problems:
+        cache, batch, q, _ = p.place(nt)
+        jobs.append((p, cache, batch, q, [torch.full_like(q, 77.0) for _ in range(15)], p.attention(True)))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(p, cache, batch, q, outs, _, prefix):
+        try:
+            for o in outs:
+                if prefix:
+                    nt.attention_prefix(cache, batch, q, o, p.scale, prefix)
+                else:
+                    nt.attention_cached(cache, batch, q, o, p.scale)
+        except Exception as e:                          # noqa: BLE001 - the main thread reports it
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(*j, prefix)) for j, prefix in zip(jobs, (0, 0, 1280))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for p, _, _, _, outs, (want, tol) in jobs:
+        for o in outs:
+            assert_within(o, want, tol, "threads")
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_pieces_of_text_recorded_and_replayed(gpu, half):
+    """Prompts appended and attended to in tiles, recorded with room for longer ones and replayed with other lengths and starts."""
+    import torch
+    heads, kv, dh, page = 8, 2, 64, 16
+    sizes = [([700, 300, 900], [200, 100, 212]), ([900, 280, 640], [30, 270, 212]), ([512, 513, 900], [170, 171, 171])]
+    p = Problem([900] * 3, [200, 100, 212], heads, kv, dh, page, half, 74)
+    cache, batch, q, out = p.place(nt)
+    p.kd.nan_to_num_()
+    p.vd.nan_to_num_()
+    batch = nt.CacheBatch(p.lengths_d, p.table_d, starts=p.starts_d, tokens=512, max_new=300, max_length=900)
+    k, v = torch.randn((512, kv, dh), device=gpu).to(q.dtype), torch.randn((512, kv, dh), device=gpu).to(q.dtype)
+
+    def step():
+        nt.cache_append(cache, batch, k, v)
+        nt.attention_cached(cache, batch, q, out, p.scale)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for turn in range(2):
+        for lens, new in sizes:
+            starts = [0]
+            for a in new:
+                starts.append(starts[-1] + a)
+            p.lengths_d.copy_(torch.tensor(lens, dtype=torch.int32))
+            p.starts_d.copy_(torch.tensor(starts, dtype=torch.int32))
+            k.normal_()
+            out.fill_(77.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = out.clone()
+            p.lens, p.new, p.starts, p.tokens = lens, new, starts, 512
+            p.k, p.v = p.kd.cpu(), p.vd.cpu()
+            want, tol = p.attention(True)
+            assert_within(got, want, tol, "replay %d" % turn)
+            step()
+            torch.cuda.synchronize()
+            assert torch.equal(got, out)
