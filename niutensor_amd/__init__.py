@@ -8,6 +8,7 @@ fallback: if the library is missing, or there is no gfx950 device, calls fail.
 """
 import ctypes as C
 import os
+import struct
 import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -354,6 +355,7 @@ class KVCache:
     [pages][heads][positions][dh] is passed as its transpose(1, 2). Keep it as long as the cache lives."""
 
     def __init__(self, k, v):
+        import torch
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise NtsAmdError("Unmatched tensors in the cache!")
         if k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
@@ -363,6 +365,9 @@ class KVCache:
         self._c = _Cache(k.data_ptr(), v.data_ptr(), _dtype_code(k), k.shape[0], k.shape[1], k.shape[2], k.shape[3],
                          (C.c_longlong * 6)(*k.stride()[:3], *v.stride()[:3]))
         self._ref = C.addressof(self._c)
+        # looked up once: a step of decoding is a few microseconds, half of them here
+        self._float = torch.float32
+        self._stream = torch._C._cuda_getCurrentRawStream if self.device >= 0 else lambda device: None
 
 
 class CacheBatch:
@@ -387,58 +392,52 @@ class CacheBatch:
         self._ref = C.addressof(self._c)
 
 
-def _rows(t, cache, batch, heads):
-    """Strides of a [tokens][heads][dh] tensor of the cache's type, on its device."""
-    if t.dtype is not cache.dtype or t.get_device() != cache.device or batch.device != cache.device:
+_strides4, _strides8 = struct.Struct("4q").pack, struct.Struct("8q").pack
+
+
+def _rows(s, t, cache, batch, heads=None):
+    """Strides of two [tokens][heads][dh] tensors of the cache's type, on its device, and their heads (default: any)."""
+    shape, dtype, device = s.shape, cache.dtype, cache.device
+    if s.dtype is not dtype or t.dtype is not dtype or s.get_device() != device or t.get_device() != device or batch.device != device:
         raise NtsAmdError("rows of the cache's data type and device are wanted")
-    s = t.stride()
-    if t.shape != (batch.tokens, heads, cache.dh) or (s[2] != 1 and cache.dh > 1):
-        raise NtsAmdError("Unmatched tensors: %s for %d tokens, %d heads of %d contiguous columns"
-                          % (tuple(t.shape), batch.tokens, heads, cache.dh))
-    return s
-
-
-def _stream_of(device):
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device) if device >= 0 else None
-
-
-_Strides4, _Strides8 = C.c_longlong * 4, C.c_longlong * 8
+    if len(shape) != 3 or t.shape != shape or shape[0] != batch.tokens or shape[2] != cache.dh or (heads is not None and shape[1] != heads):
+        raise NtsAmdError("Unmatched tensors: %s and %s for %d tokens and heads of %d columns"
+                          % (tuple(shape), tuple(t.shape), batch.tokens, cache.dh))
+    s0, s1, s2 = s.stride()
+    t0, t1, t2 = t.stride()
+    if (s2 != 1 or t2 != 1) and cache.dh > 1:
+        raise NtsAmdError("Unmatched tensors: the columns of a head must be contiguous")
+    return s0, s1, t0, t1, shape[1]
 
 
 def cache_append(cache, batch, k, v, rotation=None, pairs=False, q=None, q_out=None):
     """The new tokens' keys and values ([tokens][heads][dh], any strides) to their places in the cache; keys, and
     queries to q_out (which may be q), turned by rotation: float [positions][columns / 2][2] of cosine and sine.
     pairs: neighbouring columns are turned together, otherwise column j and j + columns / 2."""
-    ks, vs = _rows(k, cache, batch, cache.heads), _rows(v, cache, batch, cache.heads)
-    qs = os_ = ks
-    heads = 0
+    k0, k1, v0, v1, _ = _rows(k, v, cache, batch, cache.heads)
+    q0 = q1 = o0 = o1 = heads = positions = rotated = 0
     qp = op = rp = None
     if q is not None:
-        if q.dim() != 3 or q_out is None:
+        if q_out is None:
             raise NtsAmdError("Unmatched tensors: queries need a [tokens][heads][dh] result")
-        heads = q.shape[1]
-        qs, os_ = _rows(q, cache, batch, heads), _rows(q_out, cache, batch, heads)
+        q0, q1, o0, o1, heads = _rows(q, q_out, cache, batch)
         qp, op = q.data_ptr(), q_out.data_ptr()
-    positions = rotated = 0
     if rotation is not None:
-        if rotation.dim() != 3 or rotation.shape[2] != 2 or not rotation.is_contiguous() or _dtype_code(rotation) != X_FLOAT \
+        shape = rotation.shape
+        if len(shape) != 3 or shape[2] != 2 or not rotation.is_contiguous() or rotation.dtype is not cache._float \
                 or rotation.get_device() != cache.device:
             raise NtsAmdError("rotation must be a dense float [positions][columns / 2][2] tensor")
-        positions, rotated, rp = rotation.shape[0], 2 * rotation.shape[1], rotation.data_ptr()
-    _check(load().ntsamd_cache_append(cache.device, _stream_of(cache.device), cache._ref, batch._ref, k.data_ptr(), v.data_ptr(),
-                                      qp, op, heads, _Strides8(ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1]),
+        positions, rotated, rp = shape[0], 2 * shape[1], rotation.data_ptr()
+    _check(load().ntsamd_cache_append(cache.device, cache._stream(cache.device), cache._ref, batch._ref, k.data_ptr(), v.data_ptr(),
+                                      qp, op, heads, _strides8(k0, k1, v0, v1, q0, q1, o0, o1),
                                       rp, positions, rotated, ROTATE_PAIRS if pairs else ROTATE_HALVES))
     return q_out
 
 
 def _attention_rows(cache, batch, q, out):
-    if q.dim() != 3:
-        raise NtsAmdError("Unmatched tensors: queries are [tokens][heads][dh]")
-    heads = q.shape[1]
-    qs, os_ = _rows(q, cache, batch, heads), _rows(out, cache, batch, heads)
-    return (cache.device, _stream_of(cache.device), cache._ref, batch._ref, q.data_ptr(), out.data_ptr(), heads,
-            _Strides4(qs[0], qs[1], os_[0], os_[1]))
+    q0, q1, o0, o1, heads = _rows(q, out, cache, batch)
+    return (cache.device, cache._stream(cache.device), cache._ref, batch._ref, q.data_ptr(), out.data_ptr(), heads,
+            _strides4(q0, q1, o0, o1))
 
 
 def attention_cached(cache, batch, q, out, scale, causal=True):
