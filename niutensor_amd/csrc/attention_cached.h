@@ -313,6 +313,13 @@ __device__ __forceinline__ long long lane_of(long long x, int source)
     return ((long long)hi << 32) | (unsigned)lo;
 }
 
+/* lane `source`'s x, for a `source` in a scalar register, into scalar registers */
+__device__ __forceinline__ long long lane_of_all(long long x, int source)
+{
+    const int lo = __builtin_amdgcn_readlane((int)x, source), hi = __builtin_amdgcn_readlane((int)(x >> 32), source);
+    return ((long long)hi << 32) | (unsigned)lo;
+}
+
 /* entry i of a row of the page table (rows are below 4 GiB) */
 __device__ __forceinline__ int page_entry(const int * row, int i)
 {

@@ -54,7 +54,18 @@ __device__ __forceinline__ void lds_from_global16(unsigned lds, long long addres
                  : "memory");
 }
 
-/* What fetches a tile's blocks: lane l of every wave looks after key l of a block */
+/* the same from an address that the whole wave shares and an offset per lane */
+__device__ __forceinline__ void lds_from_global16(unsigned lds, long long address, unsigned offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(offset), "s"(address)
+                 : "memory");
+}
+
+/* What fetches a tile's blocks: lane l of every wave looks after key l of a block, and tells the lanes that fetch a piece of its row
+   where it stands. Where the rows that a wave fetches stand behind one another on a page, and all keys of the block are there, they
+   share an address and the lanes' offsets are the same for every block. */
 template <typename T, int DHM> struct TileFetch {
     typedef CachedTilesShared<T, DHM> Shared;
     static constexpr int KB = Shared::KB, PIECES = Shared::PIECES;
@@ -63,20 +74,22 @@ template <typename T, int DHM> struct TileFetch {
     const CachedParams & p;
     const Segment & sg;
     const int * table;
-    int lane, fetch;                        /* this lane fetches a piece of each of the rows `fetch` + ROWS s */
+    int lane, first, fetch;                 /* the wave fetches rows from `first` on; this lane fetches a piece of each of the rows `fetch` + ROWS s */
     int col[LOADS];                         /* columns past dh: the row's first, which meet zeros of q or are not stored */
     unsigned kLds, vLds;
+    unsigned kOff[LOADS], vOff[LOADS];      /* from the first of the wave's rows */
     unsigned long long there;               /* which keys of the block being fetched exist */
-    KeyPlace at;                            /* of the lane's key of that block */
 
     __device__ __forceinline__ TileFetch(const CachedParams & params, const Segment & segment, Shared & sh, int wave, int l)
         : p(params), sg(segment), table(params.c.table + (long long)segment.seq * params.c.tablePages), lane(l),
-          fetch(wave * (LOADS * ROWS) + l / PIECES), there(0)
+          first(wave * (LOADS * ROWS)), fetch(first + l / PIECES), there(0)
     {
 #pragma unroll
         for (int s = 0; s < LOADS; s++) {
             const int at = 16 * ((lane % PIECES) ^ Shared::swizzle(fetch + ROWS * s));
             col[s] = at < (int)sizeof(T) * p.c.dh ? at : 0;
+            kOff[s] = (unsigned)((lane / PIECES + ROWS * s) * (int)p.c.kR) * (unsigned)sizeof(T) + col[s];
+            vOff[s] = (unsigned)((lane / PIECES + ROWS * s) * (int)p.c.vR) * (unsigned)sizeof(T) + col[s];
         }
         kLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.k[0]) + wave * (LOADS * 1024);
         vLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.v[0]) + wave * (LOADS * 1024);
@@ -87,27 +100,30 @@ template <typename T, int DHM> struct TileFetch {
         const int key = p.first + u * KB + lane;
         return u < sg.u1 && key < sg.keys && (KB == 64 || lane < KB) ? page_entry(key < p.common ? p.c.table : table, divided(key, p.c.pageSize)) : -1;
     }
-    /* a block's fetch: look(u, ..), then loads 0 .. 2 LOADS - 1, each the address and the load itself */
-    __device__ __forceinline__ void look(int u, int page)
-    {
-        at = key_place<T>(p.c, sg.head, p.first + u * KB + lane, page);
-        there = __ballot(at.there);
-    }
-    __device__ __forceinline__ long long source(int i) const
-    {
-        const int s = i % LOADS;
-        return lane_of(i < LOADS ? at.k : at.v, fetch + ROWS * s) + col[s];
-    }
-    __device__ __forceinline__ void load(int u, int i, long long source) const
-    {
-        lds_from_global16((i < LOADS ? kLds : vLds) + ((u - sg.u0) & 1) * Shared::BLOCK + (i % LOADS) * 1024, source);
-    }
     __device__ __forceinline__ void block(int u, int page)
     {
-        look(u, page);
+        const KeyPlace at = key_place<T>(p.c, sg.head, p.first + u * KB + lane, page);
+        const unsigned stage = ((u - sg.u0) & 1) * Shared::BLOCK;
+        there = __ballot(at.there);
+        if (p.runs && there == (KB == 64 ? ~0ull : (1ull << (KB & 63)) - 1)) {
+            long long k = lane_of_all(at.k, first), v = lane_of_all(at.v, first);
+            /* registers that the vector ALU writes must have settled before a memory instruction reads them, and the compiler does not
+               see those */
+            asm volatile("s_nop 4" : "+s"(k), "+s"(v));
 #pragma unroll
-        for (int i = 0; i < 2 * LOADS; i++)
-            load(u, i, source(i));
+            for (int s = 0; s < LOADS; s++)
+                lds_from_global16(kLds + stage + s * 1024, k, kOff[s]);
+#pragma unroll
+            for (int s = 0; s < LOADS; s++)
+                lds_from_global16(vLds + stage + s * 1024, v, vOff[s]);
+            return;
+        }
+#pragma unroll
+        for (int s = 0; s < LOADS; s++)
+            lds_from_global16(kLds + stage + s * 1024, lane_of(at.k, fetch + ROWS * s) + col[s]);
+#pragma unroll
+        for (int s = 0; s < LOADS; s++)
+            lds_from_global16(vLds + stage + s * 1024, lane_of(at.v, fetch + ROWS * s) + col[s]);
     }
     /* the block being fetched has landed, for every wave, and nobody reads the other stage any more */
     __device__ __forceinline__ void landed() const

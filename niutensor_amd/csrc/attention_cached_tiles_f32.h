@@ -95,8 +95,8 @@ __device__ __forceinline__ void attend_tile_f32(const CachedParams & p, int id, 
         const char * const Ks = sh.k[(u - sg.u0) & 1];
         const char * const Vs = sh.v[(u - sg.u0) & 1];
         from.landed();
-        const bool more = u + 1 < sg.u1;
-        from.look(u + 1, page);                 /* past the last block: no page, and not fetched */
+        if (u + 1 < sg.u1)
+            from.block(u + 1, page);
         page = from.page_of(u + 2);
 
         /* ---- S^T = K Q^T ---- */
@@ -112,19 +112,12 @@ __device__ __forceinline__ void attend_tile_f32(const CachedParams & p, int id, 
             kf[0][j] = *reinterpret_cast<const f32x4 *>(&Ks[kAt[0] + 16 * j * ROW]);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            /* a step's operands are read, and some of the next block's rows are looked up and sent for, while the one before is
-               multiplied: left to itself the compiler does so right before */
-            constexpr int ALL_LOADS = 2 * TileFetch<float, DHM>::LOADS;
-            const int from0 = t * ALL_LOADS / NT, from1 = (t + 1) * ALL_LOADS / NT;
-            long long source[ALL_LOADS];
+            /* a step's operands are read while the one before is multiplied: left to itself the compiler reads them right before */
             if (t + 1 < NT) {
 #pragma unroll
                 for (int j = 0; j < NJ; j++)
                     kf[(t + 1) & 1][j] = *reinterpret_cast<const f32x4 *>(&Ks[kAt[t + 1] + 16 * j * ROW]);
             }
-#pragma unroll
-            for (int i = from0; i < from1; i++)
-                source[i] = from.source(i);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -134,10 +127,6 @@ __device__ __forceinline__ void attend_tile_f32(const CachedParams & p, int id, 
                     for (int q = 0; q < QR; q++)
                         s[q][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[t & 1][j][e], qf[q][t][e], s[q][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = from0; i < from1; i++)
-                if (more)
-                    from.load(u + 1, i, source[i]);
         }
         VPiece vf[2][NH];
 #pragma unroll

@@ -1096,6 +1096,8 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     p.acc = p.stat = NULL;
     prefix = prefix < p.c.maxLength ? prefix : p.c.maxLength;
     p.common = prefix;
+    const int runs = p.runs;
+    p.runs = runs && prefix % 16 == 0 ? 1 : 0;          /* the page in which a prefix ends may be two */
 
     if (rows > 32) {
         /* many rows to a sequence: tiles of rows and pieces of keys, whatever of both the estimate likes best */
@@ -1195,6 +1197,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 pre = o;
                 pre.mode = CACHED_TILES;
                 pre.first = 0;
+                pre.runs = runs;
                 pre.prefix = prefix;
                 /* rows of its tiles and pieces of its keys by the estimate for tiles, which is without the sequences' own keys: one
                    workgroup to a CU beside many of theirs, two beside few */
@@ -1326,6 +1329,8 @@ int attention_over_cache(int devID, void * stream, const ntsamd_cache * cache, c
     p.perDiv = fast_div(p.per);
     p.scale = scale;
     p.causal = causal != 0;
+    const long long reach = 16LL * (p.c.kR > p.c.vR ? p.c.kR : p.c.vR) * (half ? 2 : 4);
+    p.runs = cache->pageSize % 16 == 0 && reach <= 0x7fffffffLL ? 1 : 0;
     return run_attention_cached(devID, static_cast<hipStream_t>(stream), p, half, prefix);
 }
 
