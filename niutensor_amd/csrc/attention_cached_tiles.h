@@ -15,8 +15,9 @@
  * comparisons. Fetches of keys that a tile does not have read a row of zeros.
  *
  * A wave's block of 64 keys, 32 rows and 128 columns is 1090 cycles of MFMAs and about as many of vector instructions, 512 of them
- * exponentials. 4 pieces of text of 257 to 1024 tokens in sequences of 1500 to 4096, 32 heads on 8 of 128: 133 us, 735 TFLOP/s with
- * the last round of workgroups half empty; 860 at large even lengths (a large product reaches 1207).
+ * exponentials. 4 pieces of text of 257 to 1024 tokens in sequences of 1500 to 4096, 32 heads on 8 of 128: 121 us, 807 TFLOP/s with
+ * the last round of workgroups half empty; 959 for 8 times 1024 on 4096 (837, 783, 529 with heads of 96, 64, 32; a large product
+ * reaches 1207).
  */
 #pragma once
 #include "gemm_common.h"
@@ -54,18 +55,21 @@ __device__ __forceinline__ void lds_from_global16(unsigned lds, long long addres
                  : "memory");
 }
 
-/* the same from an address that the whole wave shares and an offset per lane */
+/* the same from an address that the whole wave shares and an offset per lane. A memory instruction must not read a scalar register
+   within five cycles of the vector ALU writing it, which the compiler sees to only for its own */
 __device__ __forceinline__ void lds_from_global16(unsigned lds, long long address, unsigned offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(lds), "v"(offset), "s"(address)
                  : "memory");
 }
 
 /* What fetches a tile's blocks: lane l of every wave looks after key l of a block, and tells the lanes that fetch a piece of its row
-   where it stands. Where the rows that a wave fetches stand behind one another on a page, and all keys of the block are there, they
-   share an address and the lanes' offsets are the same for every block. */
+   where it stands. Where all keys of a block are there, the rows that a wave fetches with one load stand behind one another on a
+   page, if that has a multiple of their number: they share an address, and the lanes' offsets are the same for every block. With
+   pages of a multiple of 16 positions all rows of a wave do (4 pieces of text of 257 to 1024 tokens in sequences of 1500 to 4096, 32
+   heads on 8 of 128, half, pages of 64: 133 us with an address per row, 121 so). */
 template <typename T, int DHM> struct TileFetch {
     typedef CachedTilesShared<T, DHM> Shared;
     static constexpr int KB = Shared::KB, PIECES = Shared::PIECES;
@@ -88,8 +92,8 @@ template <typename T, int DHM> struct TileFetch {
         for (int s = 0; s < LOADS; s++) {
             const int at = 16 * ((lane % PIECES) ^ Shared::swizzle(fetch + ROWS * s));
             col[s] = at < (int)sizeof(T) * p.c.dh ? at : 0;
-            kOff[s] = (unsigned)((lane / PIECES + ROWS * s) * (int)p.c.kR) * (unsigned)sizeof(T) + col[s];
-            vOff[s] = (unsigned)((lane / PIECES + ROWS * s) * (int)p.c.vR) * (unsigned)sizeof(T) + col[s];
+            kOff[s] = (unsigned)(lane / PIECES + ROWS * s) * (unsigned)p.c.kR * (unsigned)sizeof(T) + col[s];
+            vOff[s] = (unsigned)(lane / PIECES + ROWS * s) * (unsigned)p.c.vR * (unsigned)sizeof(T) + col[s];
         }
         kLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.k[0]) + wave * (LOADS * 1024);
         vLds = (unsigned)(size_t)((__attribute__((address_space(3))) char *)sh.v[0]) + wave * (LOADS * 1024);
@@ -105,17 +109,24 @@ template <typename T, int DHM> struct TileFetch {
         const KeyPlace at = key_place<T>(p.c, sg.head, p.first + u * KB + lane, page);
         const unsigned stage = ((u - sg.u0) & 1) * Shared::BLOCK;
         there = __ballot(at.there);
-        if (p.runs && there == (KB == 64 ? ~0ull : (1ull << (KB & 63)) - 1)) {
-            long long k = lane_of_all(at.k, first), v = lane_of_all(at.v, first);
-            /* registers that the vector ALU writes must have settled before a memory instruction reads them, and the compiler does not
-               see those */
-            asm volatile("s_nop 4" : "+s"(k), "+s"(v));
+        if (p.runs >= ROWS && there == (KB == 64 ? ~0ull : (1ull << (KB & 63)) - 1)) {
+            if (p.runs >= LOADS * ROWS) {
+                const long long k = lane_of_all(at.k, first), v = lane_of_all(at.v, first);
+#pragma unroll
+                for (int s = 0; s < LOADS; s++)
+                    lds_from_global16(kLds + stage + s * 1024, k, kOff[s]);
+#pragma unroll
+                for (int s = 0; s < LOADS; s++)
+                    lds_from_global16(vLds + stage + s * 1024, v, vOff[s]);
+                return;
+            }
+            const unsigned kStep = ROWS * (unsigned)p.c.kR * (unsigned)sizeof(T), vStep = ROWS * (unsigned)p.c.vR * (unsigned)sizeof(T);
 #pragma unroll
             for (int s = 0; s < LOADS; s++)
-                lds_from_global16(kLds + stage + s * 1024, k, kOff[s]);
+                lds_from_global16(kLds + stage + s * 1024, lane_of_all(at.k, first + ROWS * s), kOff[s] - s * kStep);
 #pragma unroll
             for (int s = 0; s < LOADS; s++)
-                lds_from_global16(vLds + stage + s * 1024, v, vOff[s]);
+                lds_from_global16(vLds + stage + s * 1024, lane_of_all(at.v, first + ROWS * s), vOff[s] - s * vStep);
             return;
         }
 #pragma unroll

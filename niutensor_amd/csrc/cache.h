@@ -97,7 +97,7 @@ struct CachedParams {
     int groups;                         /* CACHED_PIECES: pieces aimed at; CACHED_TILES: pieces of a tile's keys */
     int tiles;                          /* CACHED_TILES: tiles launched (at least those that the batch can have) */
     int sorted;                         /* CACHED_WHOLE, and CACHED_TILES without partial results, up to 64 sequences: the longest first */
-    int runs;                           /* CACHED_TILES: 16 keys from a multiple of 16 on are on one page, 2 GiB at most */
+    int runs;                           /* CACHED_TILES: so many keys (16, or 8, 4, 2) from a multiple of it on are on one page, within 2 GiB */
     int rows;                           /* rows of a slot */
     /* partial results: acc[slot][row][dh] and stat[slot][row][2] (maximum and sum, base 2); NULL: results go to out */
     float * acc;

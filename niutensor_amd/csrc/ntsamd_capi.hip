@@ -1097,7 +1097,8 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
     prefix = prefix < p.c.maxLength ? prefix : p.c.maxLength;
     p.common = prefix;
     const int runs = p.runs;
-    p.runs = runs && prefix % 16 == 0 ? 1 : 0;          /* the page in which a prefix ends may be two */
+    while (p.runs > 1 && prefix % p.runs != 0)          /* the page in which a prefix ends may be two */
+        p.runs /= 2;
 
     if (rows > 32) {
         /* many rows to a sequence: tiles of rows and pieces of keys, whatever of both the estimate likes best */
@@ -1330,7 +1331,11 @@ int attention_over_cache(int devID, void * stream, const ntsamd_cache * cache, c
     p.scale = scale;
     p.causal = causal != 0;
     const long long reach = 16LL * (p.c.kR > p.c.vR ? p.c.kR : p.c.vR) * (half ? 2 : 4);
-    p.runs = cache->pageSize % 16 == 0 && reach <= 0x7fffffffLL ? 1 : 0;
+    p.runs = 16;
+    while (p.runs > 1 && cache->pageSize % p.runs != 0)
+        p.runs /= 2;
+    if (reach > 0x7fffffffLL)
+        p.runs = 0;
     return run_attention_cached(devID, static_cast<hipStream_t>(stream), p, half, prefix);
 }
 
