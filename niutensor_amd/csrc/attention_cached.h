@@ -168,7 +168,7 @@ __device__ __forceinline__ Segment tile_segment(const CachedParams & p, CachedSc
 {
     /* the last tiles of a sequence see the most keys: first. Where there are more workgroups than run at once, those of the longest
        sequence too, so that the last ones to start are short (4 pieces of text of 257 to 1024 tokens in sequences of 1500 to 4096,
-       32 heads on 8 of 128, half: 142 us in the order of the batch, 134 so) */
+       32 heads on 8 of 128, half: 142 us in the order of the batch, 134 so, both with an address per row) */
     const int perTile = p.c.kvHeads * p.groups;
     const int tile = p.tiles - 1 - id / perTile, rest = id % perTile, piece = rest / p.c.kvHeads;
     int start, fresh, length, keys, seq = 0, row0 = tile * TR;
