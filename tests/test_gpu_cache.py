@@ -437,6 +437,20 @@ def test_prefix_of_any_length(gpu, half, prefix):
     assert_within(out, want, tol, nt.last_plan())
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("prefix", [1010, 1012, 1015])
+@pytest.mark.parametrize("new,heads,kv", [(1, 4, 2), (40, 4, 2), (120, 32, 4)])
+@pytest.mark.parametrize("dh", [32, 64, 128])
+def test_page_in_which_a_prefix_ends(gpu, half, prefix, new, heads, kv, dh):
+    """Every sequence has a page of its own there, of which only what follows the prefix counts; one or many new tokens."""
+    p = Problem([1060, 1100, 1071], [new] * 3, heads, kv, dh, 16, half, 27, prefix=1008)
+    p.row = lambda i, pos: (int(p.table[0 if pos < prefix else i, pos // 16]), pos % 16)
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    assert_within(out, want, tol, nt.last_plan())
+
+
 def test_prefix_is_read_through_the_first_row_of_the_table(gpu):
     """The other sequences' entries for the prefix are not looked at."""
     p = Problem([140, 150, 160], [1, 1, 1], 4, 2, 64, 16, True, 22, prefix=128, uniform=True)
