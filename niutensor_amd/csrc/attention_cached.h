@@ -14,11 +14,26 @@ struct CachedScan {
     int order[64];
 };
 
+/* Keys that the kernels take at a time: a wave of the few-rows kernel, a workgroup of tiles of 64 rows and more */
+constexpr int CACHED_TILE_KEYS = 64;
+constexpr int cached_block_keys(bool half, int columns, int rows)
+{
+    return rows < 64 ? (half ? 32 : 16) : (!half && columns > 64 ? 32 : CACHED_TILE_KEYS);
+}
+
+/* The first position that a sequence's own launch takes. A sequence that ends inside the shared prefix has no use for the partial
+   result of the piece in which it ends: what stands behind its end is multiplied there too, by probabilities of zero, which is NaN
+   where it is not finite. It takes the pieces that it has whole, and reads the rest, less than a piece, for itself. */
+__device__ __forceinline__ int first_of(const CachedParams & p, const CacheSequence & s)
+{
+    return s.length >= p.first ? p.first : divided(s.length, p.part) * (int)p.part.d;
+}
+
 /* units of keys of one (sequence, key head) pair: at least one where there are tokens to answer */
 template <int UK>
 __device__ __forceinline__ int units_of(const CachedParams & p, const CacheSequence & s)
 {
-    return s.fresh > 0 ? max((max(s.length - p.first, 0) + UK - 1) / UK, 1) : 0;
+    return s.fresh > 0 ? max((s.length - first_of(p, s) + UK - 1) / UK, 1) : 0;
 }
 
 /* Sums over the sequences of a launch, weight(i) each: every thread of the 64 NW takes a run of sequences. */
@@ -117,7 +132,8 @@ struct Segment {
     int seq, head;                      /* table row, key head */
     int row0, rows;                     /* first row of the tile, rows the sequence has (0: nothing to do) */
     int keys;                           /* positions that any row of the tile sees */
-    int u0, u1;                         /* units, from p.first on */
+    int first;                          /* position at which the units begin */
+    int u0, u1;                         /* units */
     int slot;                           /* where the partial result goes, -1: the result goes to out */
 };
 
@@ -133,6 +149,7 @@ __device__ __forceinline__ Segment uniform(Segment sg)
     sg.row0 = __builtin_amdgcn_readfirstlane(sg.row0);
     sg.rows = __builtin_amdgcn_readfirstlane(sg.rows);
     sg.keys = __builtin_amdgcn_readfirstlane(sg.keys);
+    sg.first = __builtin_amdgcn_readfirstlane(sg.first);
     sg.u0 = __builtin_amdgcn_readfirstlane(sg.u0);
     sg.u1 = __builtin_amdgcn_readfirstlane(sg.u1);
     sg.slot = __builtin_amdgcn_readfirstlane(sg.slot);
@@ -194,7 +211,12 @@ __device__ __forceinline__ Segment tile_segment(const CachedParams & p, CachedSc
         if (p.causal)
             keys -= fresh - 1 - divided(max(min(row0 + TR, fresh * p.per) - 1, 0), p.perDiv);
     }
-    const int units = (max(keys - p.first, 0) + UK - 1) / UK, each = (units + p.groups - 1) / p.groups;
+    const int units = (max(keys, 0) + UK - 1) / UK;
+    int each = units;
+    if (p.prefix > 0)
+        each = (int)p.part.d / UK;
+    else if (p.groups > 1)
+        each = (units + p.groups - 1) / p.groups;
     Segment sg;
     sg.s.start = start;
     sg.s.fresh = fresh;
@@ -204,6 +226,7 @@ __device__ __forceinline__ Segment tile_segment(const CachedParams & p, CachedSc
     sg.row0 = row0;
     sg.rows = row0 < fresh * p.per ? fresh * p.per : 0;
     sg.keys = keys;
+    sg.first = 0;
     sg.u0 = min(each * piece, units);
     sg.u1 = min(sg.u0 + each, units);
     sg.slot = p.acc ? (tile * p.c.kvHeads + sg.head) * p.groups + piece : -1;
@@ -339,7 +362,6 @@ int launch_attention_pairs(const CachedParams & p, bool half, int tile, bool wid
    waves share out the keys */
 int launch_attention_tiles(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream);
 int launch_attention_tile_rows(const CachedParams & p, bool half, int tile, int blocks, hipStream_t stream);
-constexpr int CACHED_TILE_KEYS = 64;
 /* both launches of a shared prefix in one: `pre` over it in tiles of `tile` rows (64 or 128 half, 16, 32 or 64 float), `own` over each
    sequence's own keys, 16 qr rows */
 int launch_attention_prefix(const CachedParams & pre, const CachedParams & own, bool half, int tile, int qr, int preBlocks,

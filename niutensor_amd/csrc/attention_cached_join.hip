@@ -72,7 +72,7 @@ attention_join_kernel(const JoinParams j)
             const int tile = r / j.preRows;
             preRow = r - tile * j.preRows;
             preSlot = (tile * kv + head) * j.prePieces;
-            pre = j.prePieces;
+            pre = s.length >= p.first ? j.prePieces : divided(s.length, p.part);        /* see first_of */
         }
     }
 

@@ -36,7 +36,7 @@ namespace ntsamd {
 
 template <typename T, int DHM> struct Unit;
 template <int DHM> struct Unit<half_t, DHM> {
-    static constexpr int UK = 32, NJ = 2;               /* keys, blocks of 16 of them */
+    static constexpr int UK = cached_block_keys(true, DHM, 16), NJ = UK / 16;   /* keys, blocks of 16 of them */
     static constexpr int NT = DHM / 32;                 /* 16-byte pieces of a key row per lane */
     static constexpr int NV = 8;                        /* keys whose values a lane loads */
     static constexpr int VC = DHM / 16, NH = 1;         /* neighbouring columns of them, sets of such columns */
@@ -44,7 +44,7 @@ template <int DHM> struct Unit<half_t, DHM> {
     typedef half_t VPiece __attribute__((ext_vector_type(VC)));
 };
 template <int DHM> struct Unit<float, DHM> {
-    static constexpr int UK = 16, NJ = 1;
+    static constexpr int UK = cached_block_keys(false, DHM, 16), NJ = UK / 16;
     static constexpr int NT = DHM / 16;
     static constexpr int NV = 4;
     static constexpr int VC = DHM % 64 == 0 ? 4 : 2, NH = DHM / 16 / VC;
@@ -98,7 +98,7 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     const int * table = c.table + (long long)sg.seq * c.tablePages;
     const int myKey = lane & (U::UK - 1);
     auto page_of = [&](int u) {
-        const int key = p.first + u * U::UK + myKey;
+        const int key = sg.first + u * U::UK + myKey;
         return u < sg.u1 && key < sg.keys ? page_entry(key < p.common ? c.table : table, divided(key, c.pageSize)) : -1;
     };
     /* byte offsets of a lane's columns in a row. Columns past dh read the row's first: a key's meet zeros of q, a value's
@@ -111,7 +111,7 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
     for (int h = 0; h < U::NH; h++)
         vCol[h] = U::VC * (16 * h + m) < dh ? U::VC * (16 * h + m) * (int)sizeof(T) : 0;
     auto load = [&](int u, int page, UnitData<T, DHM> & d) {
-        const KeyPlace at = key_place<T>(c, sg.head, p.first + u * U::UK + myKey, page);
+        const KeyPlace at = key_place<T>(c, sg.head, sg.first + u * U::UK + myKey, page);
         d.there = (unsigned)__ballot(at.there) & ALL;
 #pragma unroll
         for (int j = 0; j < U::NJ; j++) {
@@ -210,7 +210,7 @@ __device__ __forceinline__ void attend(const CachedParams & p, const Segment & s
                     }
                 }
 
-        const int key0 = p.first + u * U::UK;
+        const int key0 = sg.first + u * U::UK;
         const bool cut = d.there != ALL || key0 + U::UK > seenMin;
         T pr[QR][U::NJ][4];                             /* the probabilities as the second product's operand */
 #pragma unroll
@@ -379,7 +379,8 @@ __device__ __forceinline__ Segment pair_segment(const CachedParams & p, CachedSc
     sg.rows = u1 < 0 ? 0 : sg.s.fresh * p.per;
     sg.keys = sg.s.length;
     sg.u0 = u0;
-    sg.u1 = min(u1, (max(sg.s.length - p.first, 0) + UK - 1) / UK);
+    sg.first = first_of(p, sg.s);
+    sg.u1 = min(u1, (sg.s.length - sg.first + UK - 1) / UK);
     sg.slot = slot;
     return sg;
 }

@@ -32,7 +32,7 @@ namespace ntsamd {
    swizzled by the row instead, so that 16 rows read at one column, and in half the pairs of pieces that a transposing read takes of
    8 rows, spread over all banks. */
 template <typename T, int DHM> struct CachedTilesShared {
-    static constexpr int KB = sizeof(T) == 4 && DHM > 64 ? 32 : 64;
+    static constexpr int KB = cached_block_keys(sizeof(T) == 2, DHM, 64);
     static constexpr int PIECES = DHM * (int)sizeof(T) / 16, ROW = DHM * (int)sizeof(T), BLOCK = KB * ROW;
     __attribute__((aligned(1024))) char k[2][BLOCK];
     __attribute__((aligned(1024))) char v[2][BLOCK];
@@ -101,12 +101,12 @@ template <typename T, int DHM> struct TileFetch {
     /* the page of the lane's key of block u */
     __device__ __forceinline__ int page_of(int u) const
     {
-        const int key = p.first + u * KB + lane;
+        const int key = u * KB + lane;
         return u < sg.u1 && key < sg.keys && (KB == 64 || lane < KB) ? page_entry(key < p.common ? p.c.table : table, divided(key, p.c.pageSize)) : -1;
     }
     __device__ __forceinline__ void block(int u, int page)
     {
-        const KeyPlace at = key_place<T>(p.c, sg.head, p.first + u * KB + lane, page);
+        const KeyPlace at = key_place<T>(p.c, sg.head, u * KB + lane, page);
         const unsigned stage = ((u - sg.u0) & 1) * Shared::BLOCK;
         there = __ballot(at.there);
         if (p.runs >= ROWS && there == (KB == 64 ? ~0ull : (1ull << (KB & 63)) - 1)) {
@@ -235,7 +235,7 @@ __device__ __forceinline__ void attend_tile(const CachedParams & p, int id, Cach
         vAt[d] = trRow * (2 * DHM) + 16 * ((2 * d + ((m & 3) >> 1)) ^ Shared::swizzle(trRow)) + 8 * (m & 1);
 
     for (int u = sg.u0; u < sg.u1; u++) {
-        const int key0 = p.first + u * KB;
+        const int key0 = u * KB;
         const unsigned long long exist = from.there;
         const char * const Ks = sh.k[(u - sg.u0) & 1];
         const char * const Vs = sh.v[(u - sg.u0) & 1];

@@ -90,7 +90,7 @@ __device__ __forceinline__ void attend_tile_f32(const CachedParams & p, int id, 
         }
 
     for (int u = sg.u0; u < sg.u1; u++) {
-        const int key0 = p.first + u * KB;
+        const int key0 = u * KB;
         const unsigned long long exist = from.there;
         const char * const Ks = sh.k[(u - sg.u0) & 1];
         const char * const Vs = sh.v[(u - sg.u0) & 1];

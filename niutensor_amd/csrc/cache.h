@@ -90,7 +90,7 @@ struct CachedParams {
     float scale;
     int causal;
     int seq0, seqs;                     /* the sequences of this launch: seq0 .. seq0 + seqs - 1 */
-    int first;                          /* positions before this one are another launch's (the shared prefix) */
+    int first;                          /* positions before this one are another launch's (the shared prefix), see first_of */
     int common;                         /* positions before this one are found through the first row of the table */
     int prefix;                         /* > 0: this launch is the shared prefix of that many positions */
     int mode;                           /* CachedMode */
@@ -103,6 +103,7 @@ struct CachedParams {
     float * acc;
     float * stat;
     int * slots;                        /* CACHED_PIECES: first slot and number of pieces of every pair, for the join */
+    FastDiv part;                       /* with a shared prefix: keys of its pieces but the last */
 };
 
 /* CACHED_WHOLE: a workgroup takes all keys of one (sequence, key head).

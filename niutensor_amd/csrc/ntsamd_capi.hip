@@ -1192,7 +1192,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             o.seqs = n - seq0 < step ? n - seq0 : step;
             o.first = prefix;
             const long long pairs = (long long)o.seqs * kv;
-            long long used = 0, preBlocks = 0;
+            long long used = 0, preBlocks = 0, ownMost = own;
             if (withPrefix) {
                 const long long all = o.seqs * rows;
                 pre = o;
@@ -1222,7 +1222,12 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 }
                 pre.tiles = (int)((all + pre.rows - 1) / pre.rows);
                 const long long slots = (long long)pre.tiles * kv;
-                pre.groups = (int)pieces;
+                /* whole blocks to a piece; what that leaves of the last pieces is none */
+                const int block = cached_block_keys(half, dh, pre.rows);
+                const int part = (int)(((prefix + block - 1) / block + pieces - 1) / pieces) * block;
+                pre.groups = (prefix + part - 1) / part;
+                pre.part = o.part = fast_div(part);
+                ownMost = own > part - 1 ? own : part - 1;              /* of a sequence that ends inside the prefix */
                 preBlocks = slots * pre.groups;
                 used = preBlocks * pre.rows;
                 pre.acc = work.mem;
@@ -1242,7 +1247,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                 if (groups >= cus / 2) {
                     o.mode = CACHED_PIECES;
                     o.groups = (int)groups;
-                    const long long most = pairs * ((units(own) + 3) / 4);
+                    const long long most = pairs * ((units(ownMost) + 3) / 4);
                     blocks = groups + pairs < most ? groups + pairs : most;
                 }
             }

@@ -1,0 +1,74 @@
+"""The cache's operators at the limits of what a batch may hold: what stands beyond a sequence's end, whatever its bits, in a prefix that
+others share. Against the definitions in 64 bits (tests/cache_reference.py)."""
+import math
+
+import pytest
+
+import niutensor_amd as nt
+from cache_reference import Problem, assert_within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def name_the_case(request):
+    print("\n[gpu-case] %s" % request.node.nodeid, flush=True)
+    yield
+    nt.tuning_set("NTSAMD_SPLIT_K", None)
+
+
+# ---- a prefix of which some sequences have a part only ------------------------------------------------------------
+
+BEHIND = [
+    # sequences, new tokens, prefix, heads, kv, dh, half: rows of the prefix's tiles
+    ((6, 1, 512, 4, 4, 32, False), 16),
+    ((6, 1, 512, 4, 4, 128, False), 16),
+    ((6, 4, 2048, 32, 4, 64, False), 32),
+    ((6, 4, 2048, 64, 8, 96, False), 32),
+    ((20, 4, 1024, 32, 4, 64, False), 64),
+    ((20, 4, 512, 64, 8, 128, False), 64),
+    ((6, 1, 512, 4, 4, 64, True), 64),
+    ((6, 1, 520, 4, 4, 128, True), 64),
+    ((20, 4, 2048, 32, 4, 96, True), 128),
+    ((20, 4, 2048, 64, 8, 64, True), 128),
+]
+
+
+@pytest.mark.parametrize("sizes,rows", BEHIND)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("short", ["some", "the first", "all"])
+@pytest.mark.parametrize("bound", ["tight", "loose"])
+def test_what_a_prefix_holds_beyond_a_sequence(gpu, sizes, rows, bad, short, bound):
+    """From position `end` on the prefix is not finite. Sequences that end there or before never see it, whoever shares the prefix, and
+    with nobody there who has it all."""
+    n, new, prefix, heads, kv, dh, half = sizes
+    end = prefix // 3 + 7
+    lens = [(end, 0, end - 1, 1, end // 64 * 64, end // 2)[i % 6] if short == "all" or (i % 2 == 0) == (short == "the first") else prefix + 30 - i
+            for i in range(n)]
+    p = Problem(lens, [new] * n, heads, kv, dh, 8, half, 81, layout="heads" if dh % 64 else "rows", prefix=prefix, uniform=new == 1, pad_tokens=1,
+                slack=prefix // 8 + (8 if bound == "tight" else 400), max_length=prefix + 30 if bound == "tight" else 0)
+    for at in range(end, prefix):
+        page, row = p.row(0, at)
+        p.k[page, row], p.v[page, row] = bad, bad
+    cache, batch, q, out = p.place(nt)
+    nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    assert "prefix" in nt.last_plan() and (bound == "loose" or "x%d pieces=" % rows in nt.last_plan()), nt.last_plan()
+    want, tol = p.attention(True)
+    mine = [t for i in range(n) if lens[i] <= end for t in range(p.starts[i], p.starts[i + 1])] + [p.tokens - 1]
+    assert_within(out[mine], want[mine], tol[mine], nt.last_plan())
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new", [1, 3])
+def test_sequences_that_have_any_part_of_a_prefix(gpu, half, new):
+    """Lengths around every border of the prefix's pieces and blocks, all finite, with and without a causal limit; own keys in pieces."""
+    prefix = 1000
+    lens = [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 192, 250, 256, 257, 320, 384, 500, 512, 513, 640, 768, 769, 896, 960, 961, 998, 999, 1000,
+            1001, 1063, 2500]
+    p = Problem(lens, [new] * len(lens), 8, 4, 64, 8, half, 82, prefix=prefix)
+    for causal in (True, False):
+        want, tol = p.attention(causal)
+        cache, batch, q, out = p.place(nt)
+        nt.attention_prefix(cache, batch, q, out, p.scale, prefix, causal=causal)
+        assert "prefix" in nt.last_plan() and "pieces" in nt.last_plan().split()[-1], nt.last_plan()
+        assert_within(out, want, tol, nt.last_plan())
