@@ -117,10 +117,10 @@ __device__ __forceinline__ PiecePlan piece_plan(const CachedParams & p, CachedSc
 {
     PiecePlan f;
     const SequenceScan units = scan_sequences(p.seqs, sh, [&](int i) { return (long long)units_of<UK>(p, cache_sequence(p.c, p.seq0 + i)); });
-    /* whole rounds of the four waves, which take a unit each at a time */
+    /* whole rounds of the four waves, which take a unit each at a time; one where no sequence has new tokens, nor units */
     const long long total = units.total * p.c.kvHeads;
     const long long each = total >> 31 ? (total + p.groups - 1) / p.groups : ((unsigned)total + p.groups - 1) / (unsigned)p.groups;
-    f.most = (int)min((each + 3) & ~3ll, 0x7ffffffcll);
+    f.most = (int)min(max((each + 3) & ~3ll, 4ll), 0x7ffffffcll);
     __syncthreads();
     f.scan = scan_sequences(p.seqs, sh, [&](int i) { return pieces_of<UK>(p, i, f.most); });
     return f;

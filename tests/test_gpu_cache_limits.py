@@ -72,3 +72,30 @@ def test_sequences_that_have_any_part_of_a_prefix(gpu, half, new):
         nt.attention_prefix(cache, batch, q, out, p.scale, prefix, causal=causal)
         assert "prefix" in nt.last_plan() and "pieces" in nt.last_plan().split()[-1], nt.last_plan()
         assert_within(out, want, tol, nt.last_plan())
+
+
+# ---- batches without new tokens ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("max_new,prefix,plan", [(1, 0, "pieces="), (1, 512, "attention_prefix_kernel"), (40, 0, "tiles=")])
+@pytest.mark.parametrize("start", [0, 2])
+def test_a_batch_without_new_tokens(gpu, half, max_new, prefix, plan, start):
+    """All starts equal: nothing is computed, and no row is touched. One sequence with a token among such ones gets its result."""
+    n = 5
+    p = Problem([3000, 2900, 2000, 1024, 600], [1] * n, 8, 2, 64, 16, half, 83, prefix=prefix, pad_tokens=40)
+    p.max_new = max_new
+    cache, batch, q, out = p.place(nt)
+    call = (lambda: nt.attention_prefix(cache, batch, q, out, p.scale, prefix)) if prefix else (lambda: nt.attention_cached(cache, batch, q, out, p.scale))
+    p.starts_d.fill_(start)
+    call()
+    assert plan in nt.last_plan(), nt.last_plan()
+    assert (out == 77.0).all()
+    before = p.kd.clone()
+    new = q[:, :2].contiguous()
+    nt.cache_append(cache, batch, new, new)
+    assert (p.kd == before).logical_or(before.isnan()).all() and (p.kd.isnan() == before.isnan()).all()
+    p.starts_d[3:] = start + 1
+    call()
+    p.new, p.starts = [0, 0, 1, 0, 0], [start] * 3 + [start + 1] * 3
+    want, tol = p.attention(True)
+    assert_within(out, want, tol, nt.last_plan())
