@@ -33,6 +33,9 @@ __device__ __forceinline__ int divided(int n, const FastDiv & f)
     return (int)(((unsigned long long)(unsigned)n * f.mul) >> f.shift);
 }
 
+/* Workgroups of a launch: its threads are counted in 32 bits, and of one with more, workgroups are left out without an error. */
+constexpr long long most_workgroups(int threads) { return 0xffffffffLL / threads; }
+
 struct CacheParams {
     void * k;                           /* the pools */
     void * v;
@@ -77,7 +80,9 @@ struct AppendParams {
     long long kT, kH, vT, vH, qT, qH, oT, oH;
     const float * rotation;             /* NULL: nothing is turned */
     int positions, rotated, pairing;
-    int items, perWave, waves;          /* filled in by the launcher: pieces of work per token, of them per wave, waves per token */
+    bool whole;                         /* from here on filled in by plan_cache_append: items of 16 bytes, not of single columns */
+    int items, perWave, waves;          /* pieces of work per token, of them per wave, waves per token */
+    int token0;                         /* the first token of this launch */
 };
 
 struct CachedParams {
@@ -111,6 +116,8 @@ struct CachedParams {
    CACHED_TILES: rows cut into tiles (several to a sequence), the keys of a tile into `groups` pieces. */
 enum CachedMode { CACHED_WHOLE = 0, CACHED_PIECES = 1, CACHED_TILES = 2 };
 
+/* false: a token has more items than the kernel counts */
+bool plan_cache_append(AppendParams & p, bool half);
 int launch_cache_append(AppendParams p, bool half, hipStream_t stream);
 
 }  // namespace ntsamd

@@ -109,9 +109,10 @@ cache_append_kernel(const AppendParams p)
     const CacheParams & c = p.c;
     const int lane = threadIdx.x & 63;
     const int wave = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int tok = wave / p.waves, part = wave - tok * p.waves;
-    if (tok >= c.tokens)
+    const int at = wave / p.waves, part = wave - at * p.waves;
+    if (at >= c.tokens - p.token0)
         return;
+    const int tok = p.token0 + at;
     /* the token's sequence: the last one that starts at or before it */
     int seq, place;
     if (c.starts) {
@@ -169,23 +170,37 @@ cache_append_kernel(const AppendParams p)
     }
 }
 
-template <typename T, int N>
-int launch(AppendParams p, hipStream_t stream)
+template <int N>
+bool deal_items(AppendParams & p)
 {
     const int turned = turned_pieces<N>(p), perRow = turned + (p.c.dh - (p.rotation ? p.rotated : 0)) / N;
-    p.items = p.c.kvHeads * (perRow + p.c.dh / N) + (p.q ? p.heads * perRow : 0);
+    const long long items = (long long)p.c.kvHeads * (perRow + p.c.dh / N) + (p.q ? (long long)p.heads * perRow : 0);
+    if (items > 0x7fffff00LL)                           /* ends of a wave's items are counted in 31 bits */
+        return false;
+    p.items = (int)items;
     /* A lane's items follow one another, each a load and a store that wait for memory: one each where the waves run at once (64 sequences
        of one token, 448 waves: 3.5 us; 4.6 with four). Beyond, what a wave does first counts, its look at the starts above all: two each
        (1 to 499 tokens of 7 sequences, float: 9.3, 7.7, 8.4 us with one, two and four; 8 prompts 48.5, 45.7, 47.5), four with more
        than 64 sequences (87 of up to 108 tokens: 13.9, 11.8, 9.9). */
     const int looks = p.c.starts ? p.c.sequences / 64 + 1 : 1;
-    p.perWave = (long long)p.c.tokens * ((p.items + 63) / 64) * looks <= 1024 ? 64 : (looks == 1 ? 128 : 256);
-    p.waves = (p.items + p.perWave - 1) / p.perWave;
-    const long long blocks = ((long long)p.c.tokens * p.waves + 3) / 4;
-    if (blocks > 0x1fffffffLL)                          /* the kernel counts waves in 32 bits */
-        return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((cache_append_kernel<T, N>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-    return (int)hipGetLastError();
+    p.perWave = (long long)p.c.tokens * ((items + 63) / 64) * looks <= 1024 ? 64 : (looks == 1 ? 128 : 256);
+    p.waves = (int)((items + p.perWave - 1) / p.perWave);
+    return true;
+}
+
+template <typename T, int N>
+int launch(AppendParams p, hipStream_t stream)
+{
+    const long long most = most_workgroups(256) * 4 / p.waves;      /* tokens of a launch */
+    for (long long from = 0; from < p.c.tokens; from += most) {
+        const long long n = p.c.tokens - from < most ? p.c.tokens - from : most;
+        p.token0 = (int)from;
+        hipLaunchKernelGGL((cache_append_kernel<T, N>), dim3((unsigned)((n * p.waves + 3) / 4)), dim3(256), 0, stream, p);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess)
+            return (int)err;
+    }
+    return 0;
 }
 
 }  // namespace
@@ -205,12 +220,17 @@ static bool whole_pieces(const AppendParams & p, bool half)
     return !p.rotation || (p.pairing == 0 ? p.rotated / 2 : p.rotated) % n == 0;
 }
 
+bool plan_cache_append(AppendParams & p, bool half)
+{
+    p.whole = whole_pieces(p, half);
+    return !p.whole ? deal_items<1>(p) : (half ? deal_items<8>(p) : deal_items<4>(p));
+}
+
 int launch_cache_append(AppendParams p, bool half, hipStream_t stream)
 {
-    const bool whole = whole_pieces(p, half);
     if (half)
-        return whole ? launch<half_t, 8>(p, stream) : launch<half_t, 1>(p, stream);
-    return whole ? launch<float, 4>(p, stream) : launch<float, 1>(p, stream);
+        return p.whole ? launch<half_t, 8>(p, stream) : launch<half_t, 1>(p, stream);
+    return p.whole ? launch<float, 4>(p, stream) : launch<float, 1>(p, stream);
 }
 
 }  // namespace ntsamd

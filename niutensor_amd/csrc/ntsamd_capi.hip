@@ -1104,6 +1104,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         /* many rows to a sequence: tiles of rows and pieces of keys, whatever of both the estimate likes best */
         p.mode = CACHED_TILES;
         long long tiles = 0, pieces = 1;
+        int threads = 256;
         double best = -1.0;
         for (const TileKind & kind : g_tileKinds[half ? 1 : 0]) {
             const int tile = kind.rows;
@@ -1126,6 +1127,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
                     tiles = of;
                     pieces = cut;
                     p.rows = tile;
+                    threads = kind.threads;
                 }
             }
         }
@@ -1134,7 +1136,7 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             if (work.mem == NULL)
                 pieces = 1;
         }
-        if (tiles * kv * pieces > 0x7fffffffLL || tiles * p.rows > 0x7fffffffLL || (pieces > 1 && tiles * kv * p.rows > 0x7fffffffLL))
+        if (tiles * kv * pieces > most_workgroups(threads) || tiles * p.rows > 0x7fffffffLL)
             return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
         p.tiles = (int)tiles;
         p.groups = (int)pieces;
@@ -1184,12 +1186,15 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
             const long long most = room / 4 / (rows * kv);
             step = most < n ? (most > 1 ? (int)most : 1) : n;
         }
-        if ((long long)step * kv * rows > 0x7fffffffLL / 64)
+        /* no more pairs and rows, a workgroup each, than half of what a launch takes: pieces are a few thousand more */
+        const long long fit = most_workgroups(256) / 2 / (rows * kv);
+        if (fit == 0)
             return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
-        for (int seq0 = 0; seq0 < n && rc == 0; seq0 += step) {
+        step = step < fit ? step : (int)fit;
+        for (long long seq0 = 0; seq0 < n && rc == 0; seq0 += step) {
             CachedParams o = p, pre;                    /* each sequence's own keys; the prefix */
-            o.seq0 = seq0;
-            o.seqs = n - seq0 < step ? n - seq0 : step;
+            o.seq0 = (int)seq0;
+            o.seqs = n - seq0 < step ? (int)(n - seq0) : step;
             o.first = prefix;
             const long long pairs = (long long)o.seqs * kv;
             long long used = 0, preBlocks = 0, ownMost = own;
@@ -1895,6 +1900,8 @@ int ntsamd_cache_append(int devID, void * stream, const ntsamd_cache * cache, co
     p.positions = positions;
     p.rotated = rotation ? rotated : 0;
     p.pairing = pairing;
+    if (!plan_cache_append(p, half))
+        return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
     snprintf(g_plan, sizeof(g_plan), "cache_append_kernel");
     if (planOnly)
         return NTSAMD_OK;

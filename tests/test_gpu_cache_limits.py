@@ -99,3 +99,43 @@ def test_a_batch_without_new_tokens(gpu, half, max_new, prefix, plan, start):
     p.new, p.starts = [0, 0, 1, 0, 0], [start] * 3 + [start + 1] * 3
     want, tol = p.attention(True)
     assert_within(out, want, tol, nt.last_plan())
+
+
+# ---- more workgroups than a launch may have ---------------------------------------------------------------------------
+
+def test_more_tokens_than_a_launch_takes(gpu):
+    """2^26 and some tokens of one row of keys and of values: a wave each, four to a workgroup, of which a launch has 2^24 at most."""
+    import torch
+    tokens, page = (1 << 26) + 77, 1 << 16
+    pages = -(-tokens // page)
+    kd, vd = (torch.zeros((pages, page, 1, 4), device=gpu) for _ in range(2))
+    k, v = (torch.arange(tokens * 4, dtype=torch.int32, device=gpu).view(torch.float32).view(tokens, 1, 4) for _ in range(2))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu)                 # noqa: E731
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(84))
+    batch = nt.CacheBatch(i32([tokens]), order.to(torch.int32).to(gpu)[None], tokens=tokens, max_new=tokens)
+    nt.cache_append(nt.KVCache(kd, vd), batch, k, v)
+    for got, put in ((kd, k), (vd, v)):
+        got = got[order.to(gpu)].view(-1, 1, 4)
+        assert torch.equal(got[:tokens].view(torch.int32), put.view(torch.int32)) and (got[tokens:] == 0).all()
+
+
+@pytest.mark.parametrize("length", [1, 300])
+def test_more_sequences_than_a_launch_takes(gpu, length):
+    """2^24 and some sequences of one token, all on the same pages; short ones are left whole, long ones cut into pieces and joined."""
+    import torch
+    n, page = (1 << 24) + 3, 300
+    g = torch.Generator().manual_seed(85)
+    k, v = (torch.randn((1, page, 1, 8), generator=g).half() for _ in range(2))
+    kinds = torch.randn((64, 1, 8), generator=g).half()
+    cache = nt.KVCache(k.to(gpu), v.to(gpu))
+    batch = nt.CacheBatch(torch.full((n,), length, dtype=torch.int32, device=gpu), torch.zeros((n, 1), dtype=torch.int32, device=gpu))
+    q = kinds.to(gpu).repeat(n // 64 + 1, 1, 1)[:n].contiguous()
+    out = torch.full_like(q, 77.0)
+    nt.attention_cached(cache, batch, q, out, 0.5)
+    p = Problem([length], [1], 1, 1, 8, page, True, 85, uniform=True)
+    p.k, p.v, p.scale, p.table = k, v, 0.5, p.table * 0
+    for i in range(64):
+        p.q = kinds[i:i + 1]
+        want, tol = p.attention(True)
+        lo, hi = (want - tol).to(gpu), (want + tol).to(gpu)
+        assert ((out[i::64].double() >= lo) & (out[i::64].double() <= hi)).all(), i
