@@ -1074,6 +1074,7 @@ bool cached_wide_pays(bool half, int dh, long long pairs, long long keys, int cu
 }
 
 /* How the rows and keys of a cached attention are dealt out (see attention_cached.hip for the forms). */
+constexpr int CACHED_PLAN_SEQUENCES = 2048;             /* of a launch whose keys are cut into pieces */
 constexpr int CACHED_UNIT_HALF = 32, CACHED_UNIT_FLOAT = 16;
 
 int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool half, int prefix)
@@ -1191,6 +1192,10 @@ int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool hal
         if (fit == 0)
             return fail(NTSAMD_ERR_ARGUMENT, "tensor too large");
         step = step < fit ? step : (int)fit;
+        /* to find its piece every workgroup looks at every sequence of its launch: 65536 of up to 1100 positions, one key
+           head of 64, half: 28.8 ms in one launch, 3.9, 2.7, 2.4, 2.5 ms in launches of 8192, 4096, 2048, 1024; 4096 of them: 180, 180, 180, 159, 169 us */
+        if (cut && step > CACHED_PLAN_SEQUENCES)
+            step = CACHED_PLAN_SEQUENCES;
         for (long long seq0 = 0; seq0 < n && rc == 0; seq0 += step) {
             CachedParams o = p, pre;                    /* each sequence's own keys; the prefix */
             o.seq0 = (int)seq0;

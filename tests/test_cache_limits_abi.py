@@ -49,6 +49,12 @@ def test_pairs_go_in_slices():
     assert rc == 1 and "tensor too large" in text
 
 
+def test_sequences_in_pieces_go_in_slices():
+    """Every workgroup looks at all sequences of its launch, so that a launch of many takes the square of their time."""
+    rc, plan = call("attention", 1, n=1 << 16, tokens=1 << 16, width=400)
+    assert rc == 0 and int(plan.split("pieces=")[1].split("+")[0]) <= 2048 + 512
+
+
 def test_items_of_a_token():
     """The kernel counts a token's items in 31 bits; tokens go in slices."""
     assert call("append", 1 << 29)[0] == 0

@@ -139,3 +139,16 @@ def test_more_sequences_than_a_launch_takes(gpu, length):
         want, tol = p.attention(True)
         lo, hi = (want - tol).to(gpu), (want + tol).to(gpu)
         assert ((out[i::64].double() >= lo) & (out[i::64].double() <= hi)).all(), i
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("uniform", [True, False])
+def test_more_sequences_than_a_launch_cuts_into_pieces(gpu, half, uniform):
+    n = 4500
+    p = Problem([1400 if i % 450 == 449 else 3 + i % 40 for i in range(n)], [1] * n if uniform else [i % 3 for i in range(n)], 2, 1, 8, 16, half, 86,
+                uniform=uniform)
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_cached(cache, batch, q, out, p.scale)
+    assert " pieces=" in nt.last_plan(), nt.last_plan()
+    assert_within(out, want, tol, nt.last_plan())
