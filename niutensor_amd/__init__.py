@@ -427,7 +427,8 @@ def cache_append(cache, batch, k, v, rotation=None, pairs=False, q=None, q_out=N
         if len(shape) != 3 or shape[2] != 2 or not rotation.is_contiguous() or rotation.dtype is not cache._float \
                 or rotation.get_device() != cache.device:
             raise NtsAmdError("rotation must be a dense float [positions][columns / 2][2] tensor")
-        positions, rotated, rp = shape[0], 2 * shape[1], rotation.data_ptr()
+        # a table of nothing has no address, which would stand for no table; nothing of it is read
+        positions, rotated, rp = shape[0], 2 * shape[1], rotation.data_ptr() or cache.k.data_ptr()
     _check(load().ntsamd_cache_append(cache.device, cache._stream(cache.device), cache._ref, batch._ref, k.data_ptr(), v.data_ptr(),
                                       qp, op, heads, _strides8(k0, k1, v0, v1, q0, q1, o0, o1),
                                       rp, positions, rotated, ROTATE_PAIRS if pairs else ROTATE_HALVES))

@@ -101,6 +101,29 @@ def test_a_batch_without_new_tokens(gpu, half, max_new, prefix, plan, start):
     assert_within(out, want, tol, nt.last_plan())
 
 
+# ---- tables of nothing ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("positions,rotated", [(0, 64), (0, 0), (50, 0)])
+def test_a_rotation_of_nothing(gpu, positions, rotated):
+    """Tokens beyond its positions are left out, as with any other; the others are stored as they are where no columns are turned."""
+    import torch
+    p = Problem([60, 30, 51], [20, 2, 1], 4, 2, 64, 16, True, 87)
+    cache, batch, q, out = p.place(nt)
+    p.kd.fill_(5.0)
+    p.vd.fill_(5.0)
+    k, v = torch.ones((23, 2, 64), dtype=torch.float16, device=gpu), torch.ones((23, 2, 64), dtype=torch.float16, device=gpu)
+    nt.cache_append(cache, batch, k, v, rotation=torch.zeros((positions, rotated // 2, 2), device=gpu), q=q, q_out=out)
+    at = [*range(40, 60), 28, 29, 50]
+    seq = [0] * 20 + [1] * 2 + [2]
+    want = torch.full(p.k.shape, 5.0, dtype=torch.float16)
+    for t in range(23):
+        if at[t] < positions:
+            want[p.row(seq[t], at[t])] = 1.0
+    assert torch.equal(p.kd.cpu(), want) and torch.equal(p.vd.cpu(), want)
+    there = torch.tensor([x < positions for x in at], device=gpu)
+    assert torch.equal(out[there], q[there]) and (out[~there] == 77.0).all()
+
+
 # ---- more workgroups than a launch may have ---------------------------------------------------------------------------
 
 def test_more_tokens_than_a_launch_takes(gpu):
