@@ -305,7 +305,8 @@ __device__ __forceinline__ int rows_seen(const CachedParams & p, const Segment &
 constexpr float CACHED_RISE = 8.f;
 __device__ __forceinline__ float score_scale(const CachedParams & p)
 {
-    return fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-37f);
+    const float s = fabsf(p.scale) * 1.4426950408889634f;
+    return s < 1e-37f ? 1e-37f : s;     /* no fmaxf, which would make 1e-37 of a scale that is no number */
 }
 
 /* What the positions that do not exist read: a row of the widest head. */

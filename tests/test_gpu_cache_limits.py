@@ -124,6 +124,19 @@ def test_a_rotation_of_nothing(gpu, positions, rotated):
     assert torch.equal(out[there], q[there]) and (out[~there] == 77.0).all()
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,prefix", [(1, 0), (40, 0), (1, 512)])
+def test_a_scale_that_is_not_a_number(gpu, half, new, prefix):
+    """Every score is one, and so is every result (a scale of zero would give the mean)."""
+    p = Problem([600, 545, 570], [new] * 3, 8, 2, 64, 16, half, 88, prefix=prefix)
+    cache, batch, q, out = p.place(nt)
+    if prefix:
+        nt.attention_prefix(cache, batch, q, out, math.nan, prefix)
+    else:
+        nt.attention_cached(cache, batch, q, out, math.nan)
+    assert out.isnan().all()
+
+
 # ---- more workgroups than a launch may have ---------------------------------------------------------------------------
 
 def test_more_tokens_than_a_launch_takes(gpu):
