@@ -362,7 +362,7 @@ class KVCache:
             raise NtsAmdError("the columns of the cache must be contiguous")
         self.k, self.v = k, v
         self.dtype, self.device, self.heads, self.dh = k.dtype, k.get_device(), int(k.shape[2]), int(k.shape[3])
-        self._c = _Cache(k.data_ptr(), v.data_ptr(), _dtype_code(k), k.shape[0], k.shape[1], k.shape[2], k.shape[3],
+        self._c = _Cache(k.data_ptr(), v.data_ptr(), _dtype_code(k), *_counts(*k.shape),
                          (C.c_longlong * 6)(*k.stride()[:3], *v.stride()[:3]))
         self._ref = C.addressof(self._c)
         # looked up once: a step of decoding is a few microseconds, half of them here
@@ -388,8 +388,16 @@ class CacheBatch:
         self.tokens = n * max_new if tokens is None else int(tokens)
         self.device = lengths.get_device()
         self._c = _CacheBatch(lengths.data_ptr(), starts.data_ptr() if starts is not None else None, page_table.data_ptr(),
-                              n, page_table.shape[1], self.tokens, max_new, max_length)
+                              *_counts(n, page_table.shape[1], self.tokens, max_new, max_length))
         self._ref = C.addressof(self._c)
+
+
+def _counts(*numbers):
+    """Whole numbers for 32-bit arguments, of which ctypes would silently take the low bits."""
+    for x in numbers:
+        if not -1 << 31 <= x < 1 << 31:
+            raise NtsAmdError("%d does not fit 32 bits" % x)
+    return numbers
 
 
 _strides4, _strides8 = struct.Struct("4q").pack, struct.Struct("8q").pack
@@ -451,5 +459,5 @@ def attention_cached(cache, batch, q, out, scale, causal=True):
 def attention_prefix(cache, batch, q, out, scale, prefix, causal=True):
     """attention_cached for sequences whose first `prefix` positions hold the same keys and values, which are read through
     the first row of the page table, once for all sequences."""
-    _check(load().ntsamd_attention_prefix(*_attention_rows(cache, batch, q, out), scale, 1 if causal else 0, prefix))
+    _check(load().ntsamd_attention_prefix(*_attention_rows(cache, batch, q, out), scale, 1 if causal else 0, *_counts(prefix)))
     return out

@@ -64,3 +64,18 @@ def test_items_of_a_token():
     rc, text = call("append", 1, kv=(1 << 31) - 1)
     assert rc == 1 and "tensor too large" in text
     assert call("append", 1, tokens=(1 << 31) - 1, new=(1 << 31) - 1)[0] == 0
+
+
+def test_numbers_beyond_32_bits_are_refused_by_the_binding():
+    import torch
+    lengths, table = torch.ones(2, dtype=torch.int32), torch.zeros((2, 4), dtype=torch.int32)
+    for kw in (dict(tokens=(1 << 32) + 2), dict(max_new=(1 << 32) + 1, tokens=2), dict(max_length=1 << 32), dict(max_length=(1 << 32) + 7)):
+        with pytest.raises(nt.NtsAmdError, match="32 bits"):
+            nt.CacheBatch(lengths, table, **kw)
+    k = torch.zeros((4, 16, 2, 64), dtype=torch.float16)
+    q = torch.zeros((2, 4, 64), dtype=torch.float16)
+    with pytest.raises(nt.NtsAmdError, match="32 bits"):
+        nt.attention_prefix(nt.KVCache(k, k.clone()), nt.CacheBatch(lengths, table), q, q.clone(), 1.0, (1 << 32) + 16)
+    wide = torch.zeros(1, dtype=torch.float16).expand((1 << 32) + 3, 16, 2, 1)
+    with pytest.raises(nt.NtsAmdError, match="32 bits"):
+        nt.KVCache(wide, wide)
