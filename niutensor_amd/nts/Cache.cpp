@@ -6,6 +6,12 @@
 
 namespace nts {
 
+/* an optional tensor that is given has memory: below this layer an address of NULL stands for one that is not */
+static bool HasMemory(const XTensor * t)
+{
+    return t == NULL || t->data != NULL || t->unitNum == 0;
+}
+
 /* what the entry points get of the pools and the batch; `tokens` rows of x, of `width` columns */
 static void Describe(const XTensor * keys, const XTensor * values, const AmdCacheBatch & batch, const XTensor * x,
                      ntsamd_cache & cache, ntsamd_cache_batch & b)
@@ -81,11 +87,14 @@ void _AmdCacheAppend(XTensor * keys, XTensor * values, const AmdCacheBatch & bat
         positions = rotation->dimSize[0];
         rotated = 2 * rotation->dimSize[1];
     }
+    CheckNTErrors((HasMemory(batch.starts) && HasMemory(rotation) && HasMemory(q) && HasMemory(qOut)), "Empty input tensors!");
+    /* nothing of a table without elements is read */
+    const float * turns = rotation == NULL ? NULL : (const float *)(rotation->data != NULL ? rotation->data : keys->data);
     const long long row = (long long)cache.heads * cache.dh, wide = (long long)nhead * cache.dh;
     const long long strides[8] = {row, cache.dh, row, cache.dh, wide, cache.dh, wide, cache.dh};
     int rc = ntsamd_cache_append(keys->devID, NULL, &cache, &b, k->data, v->data, q != NULL ? q->data : NULL,
                                  qOut != NULL ? qOut->data : NULL, nhead, strides,
-                                 rotation != NULL ? (const float *)rotation->data : NULL, positions, rotated,
+                                 turns, positions, rotated,
                                  isPairs ? NTSAMD_ROTATE_PAIRS : NTSAMD_ROTATE_HALVES);
     if (rc != NTSAMD_OK) {
         ShowNTErrors(ntsamd_last_error());
@@ -100,6 +109,7 @@ static void Attend(const XTensor * keys, const XTensor * values, const AmdCacheB
     Describe(keys, values, batch, q, cache, b);
     CheckNTErrors((out != NULL), "Empty input tensors!");
     const int nhead = QueryHeads(q, out, cache, b, keys->devID);
+    CheckNTErrors((HasMemory(batch.starts)), "Empty input tensors!");
     const long long wide = (long long)nhead * cache.dh;
     const long long strides[4] = {wide, cache.dh, wide, cache.dh};
     int rc = prefix < 0 ? ntsamd_attention_cached(keys->devID, NULL, &cache, &b, q->data, out->data, nhead, strides, scale, isCausal)
