@@ -137,7 +137,9 @@ XTensor AmdAttentionCached(const XTensor & keys, const XTensor & values, const A
 {
     XTensor out(q.order, q.dimSize, q.dataType, 1.0F, q.devID, q.mem);
     out.SetTMPFlag();
-    out.SetZeroAll();
+    /* without starts the first maxNew rows of every sequence are written: no fill where these are all */
+    if (batch.starts != NULL || batch.lengths == NULL || (long long)batch.lengths->unitNum * batch.maxNew < q.dimSize[0])
+        out.SetZeroAll();
     _AmdAttentionCached(&keys, &values, batch, &q, &out, scale, isCausal);
     return out;
 }

@@ -1,12 +1,13 @@
 /*
  * Tests of the cache on pages in the nts:: host layer on a gfx950 GPU, beside nts_cache_tests: both types, with and without a causal
- * limit, sequences with a common beginning, and tensors without memory.
+ * limit, sequences with a common beginning, what a call does besides its kernels, and tensors without memory.
  *
  *   nts_cache_layer_tests               run everything on device 0, exit 0 if all passed
  *   nts_cache_layer_tests --abort NAME  provoke one fatal error (no GPU needed)
  */
 #include "../../niutensor_amd/nts/Cache.h"
 
+#include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -14,6 +15,14 @@
 #include <vector>
 
 using namespace nts;
+
+/* in place of the runtime's: counts the fills that the layer issues */
+static int fills = 0;
+extern "C" hipError_t hipMemset(void * dst, int value, size_t bytes)
+{
+    fills++;
+    return hipMemsetD8((hipDeviceptr_t)dst, (unsigned char)value, bytes);
+}
 
 static const int DEV = 0;
 static const int SEQS = 3, PAGE = 16, WIDTH = 40, KV = 2, HEADS = 4, DH = 16, PREFIX = 512;
@@ -158,7 +167,12 @@ static bool TestType(TENSOR_DATA_TYPE type)
     _AmdCacheAppend(keys, values, batch, kt, vt);
 
     bool ok = true;
+    fills = 0;
     XTensor each = AmdAttentionCached(*keys, *values, batch, *qt, 0.25F);
+    if (fills != 0) {
+        printf("a step whose rows are all written fills its result %d times\n", fills);
+        ok = false;
+    }
     XTensor shared(&each);
     _AmdAttentionPrefix(keys, values, batch, qt, &shared, 0.25F, PREFIX);
     for (int i = 0; i < SEQS; i++) {
