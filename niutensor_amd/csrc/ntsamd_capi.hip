@@ -1075,12 +1075,11 @@ bool cached_wide_pays(bool half, int dh, long long pairs, long long keys, int cu
 
 /* How the rows and keys of a cached attention are dealt out (see attention_cached.hip for the forms). */
 constexpr int CACHED_PLAN_SEQUENCES = 2048;             /* of a launch whose keys are cut into pieces */
-constexpr int CACHED_UNIT_HALF = 32, CACHED_UNIT_FLOAT = 16;
 
 int run_attention_cached(int devID, hipStream_t stream, CachedParams p, bool half, int prefix)
 {
-    const int unit = half ? CACHED_UNIT_HALF : CACHED_UNIT_FLOAT;
     const int kv = p.c.kvHeads, dh = p.c.dh, n = p.c.sequences;
+    const int unit = cached_block_keys(half, dh, 16);
     const long long rows = (long long)p.c.maxNew * p.per;           /* of one sequence and key head, at most */
     int cus = devID >= 0 && devID < MAX_DEVICES ? g_deviceCUs[devID].load(std::memory_order_relaxed) : 0;
     if (cus <= 0)
