@@ -74,6 +74,28 @@ def test_sequences_that_have_any_part_of_a_prefix(gpu, half, new):
         assert_within(out, want, tol, nt.last_plan())
 
 
+# ---- probabilities in half -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,heads,slack,split,plan", [
+    (1, 8, 2, None, "rows=16 whole="), (1, 8, 400, None, "rows=16 pieces="), (1, 8, 400, 1, "rows=16 wide whole="),
+    (4, 16, 2, None, "rows=32 whole="), (4, 16, 400, None, "rows=32 pieces="), (35, 4, 2, None, "attention_cached_tile_kernel tiles=")])
+@pytest.mark.parametrize("dh", [32, 64, 128])
+def test_few_rows_in_half_lose_no_bits_of_the_probabilities(gpu, new, heads, slack, split, plan, dh):
+    """They go into the second product as the sum of two halves: the first leaves 2^-11 of a probability at most, the second 2^-11 of
+    that, or 2^-25 where it is below the normal range, of probabilities whose sum, in fp32, is at least 1. So beside what fp32 leaves,
+    (2^-22 + 2^-25 n) max |v| and the rounding of the result, which is 2^-11 of it or 2^-25."""
+    p = Problem([64, 40, 47], [new] * 3, heads, 2, dh, 16, True, 89, slack=slack, max_length=0)
+    nt.tuning_set("NTSAMD_SPLIT_K", split)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_cached(cache, batch, q, out, p.scale)
+    assert plan in nt.last_plan(), nt.last_plan()
+    p.half = False                                      # the tolerance of fp32
+    want, tol = p.attention(True)
+    most = float(p.v.nan_to_num().abs().max())
+    tol = (tol + (2.0 ** -22 + 2.0 ** -25 * 64) * most) * (1 + 2.0 ** -10) + (2.0 ** -11 * want.abs()).clamp(min=2.0 ** -25) * (1 + 2.0 ** -10)
+    assert_within(out, want, tol, nt.last_plan())
+
+
 # ---- batches without new tokens ------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("half", [True, False])
