@@ -95,8 +95,9 @@ int ntsamd_cache_append(int devID, void * stream, const ntsamd_cache * cache, co
  * never used, whatever its bits. Inside a sequence, a value that is not finite reaches every token that sees it,
  * and may reach, as NaN, tokens of the same sequence and call that stand before it.
  *   strides[0], strides[1]: token and head of q; strides[2], strides[3]: of out. q and out are 16-byte aligned, their strides
- *   multiples of 4 (float) or 8 (half) elements; out overlaps nothing else. Data types, rounding and accumulation as in ntsamd_attention: half products with fp32
- *   accumulation, softmax in fp32, probabilities rounded to half before the second product.
+ *   multiples of 4 (float) or 8 (half) elements; out overlaps nothing else. Products accumulate in fp32, and the softmax is in fp32.
+ *   Half: probabilities enter the second product as the sum of two halves where no sequence has more than 32 rows (maxNew tokens times
+ *   the query heads of a key head); otherwise, and over a shared prefix, they may be rounded to one.
  * Long sequences are cut into pieces whose partial results meet in the stream's workspace (ntsamd_gemm.h) and are
  * added up by a second kernel, always in the same order; without a workspace they run in one piece.
  */
@@ -109,9 +110,11 @@ int ntsamd_attention_cached(int devID, void * stream, const ntsamd_cache * cache
  * keys and values, and are found through the first row of the page table for all of them (what the other rows have
  * there is not looked at). They are read once for all sequences: the queries of all sequences are multiplied
  * with them as the rows of one matrix; what follows the prefix is read sequence by sequence, and the two partial
- * results are joined. The result is that of ntsamd_attention_cached but for the order of the additions. A sequence
- * shorter than the prefix sees the part of it that it has. Where there is nothing to gain (one sequence, many new
- * tokens per sequence, a short prefix, no workspace) every sequence reads the prefix for itself.
+ * results are joined. The result is that of ntsamd_attention_cached but for the order of the additions and the
+ * rounding of probabilities. A sequence shorter than the prefix sees the part of it that it has, and nothing of what stands behind its
+ * end. The prefix is shared between sequences of up to 32 rows (maxNew tokens times the query heads of a key head)
+ * where a workspace is there and the prefix long enough to gain by it; otherwise every sequence reads it for itself, in
+ * batches of more new tokens also where sharing would save most of the reading.
  */
 int ntsamd_attention_prefix(int devID, void * stream, const ntsamd_cache * cache, const ntsamd_cache_batch * batch,
                             const void * q, void * out, int heads, const long long * strides,
