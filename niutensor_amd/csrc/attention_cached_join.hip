@@ -148,12 +148,15 @@ attention_join_kernel(const JoinParams j)
 template <typename T>
 int launch_type(const JoinParams & j, long long rows, hipStream_t stream)
 {
-    /* Tiles have whole eights of rows, each in the same few pieces. Pairs: few pieces are known of those whose keys are whole (2048 rows in
-       15 and one: 44.4 us the call eight rows to a workgroup, 43.0 one). */
+    /* Tiles have whole eights of rows, each in the same few pieces. Pairs whose keys are whole, behind a prefix: a row to a workgroup has
+       eight pieces at a time, eight rows to a workgroup are an eighth of the workgroups, which is faster where rows are many for the
+       pieces. The call with eight rows against one, 16 to 256 sequences, 8 to 32 heads, both types: 512 rows in 2 pieces the same,
+       in 8 8 to 10 % slower; 1024 in 4 2 to 6 % faster, in 8 2 to 11 % slower; 2048 in 4 4 to 7 % faster, in 8 0 to 3 % faster, in 15
+       the same; 4096 in 4 10 to 19 % faster, in 8 3 to 12 %. */
     const dim3 one((unsigned)rows), eight((unsigned)((rows + 7) / 8)), block(256);
     if (j.p.mode == CACHED_TILES)
         hipLaunchKernelGGL((attention_join_kernel<T, true, true>), eight, block, 0, stream, j);
-    else if (j.p.mode == CACHED_WHOLE && j.prePieces < 8 && rows >= 2048)
+    else if (j.p.mode == CACHED_WHOLE && 256LL * j.prePieces <= rows)
         hipLaunchKernelGGL((attention_join_kernel<T, false, true>), eight, block, 0, stream, j);
     else
         hipLaunchKernelGGL((attention_join_kernel<T, false, false>), one, block, 0, stream, j);
