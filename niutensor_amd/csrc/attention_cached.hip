@@ -20,7 +20,8 @@ attention_cached_kernel(const CachedParams p)
 }
 
 /* CACHED_TILES, tiles of 16 or 32 rows (more rows: attention_cached_tiles.hip). NW: 4 waves; in half 8, for calls whose workgroups all
-   run at once (float keeps the matrix unit busy with 4: 16.4 us with 4, 14.2 with 8 for 1024 keys of 32 columns, 31 and 35 of 128) */
+   run at once. Float has the form of 4 alone, which wide heads do better with (1024 keys of 128 columns: 31 us, 35 with 8) and narrow ones worse
+   (of 32: 16.4 and 14.2). */
 template <typename T, int DHM, int QR, int NW>
 __global__ void __launch_bounds__(64 * NW, NW == 8 && DHM <= 64 ? 4 : 2)
 attention_cached_tile_kernel(const CachedParams p)
