@@ -74,6 +74,107 @@ def test_sequences_that_have_any_part_of_a_prefix(gpu, half, new):
         assert_within(out, want, tol, nt.last_plan())
 
 
+FINITE = [
+    # the tiles of a prefix that a few rows make: sequences, new tokens, prefix, heads, kv, dh, half: rows of a tile
+    ((6, 1, 1000, 4, 4, 32, False), 16),
+    ((3, 1, 2048, 8, 2, 128, False), 16),
+    ((2, 2, 700, 6, 2, 88, False), 16),
+    ((6, 1, 1000, 4, 4, 32, True), 64),
+    ((3, 1, 2048, 8, 2, 128, True), 64),
+    ((2, 2, 700, 6, 2, 88, True), 64),
+]
+
+
+@pytest.mark.parametrize("sizes,rows", FINITE)
+def test_tiles_of_a_prefix_for_few_rows(gpu, sizes, rows):
+    n, new, prefix, heads, kv, dh, half = sizes
+    p = Problem([prefix + 50 - 7 * i for i in range(n)], [new] * n, heads, kv, dh, 20, half, 90, prefix=prefix, pad_tokens=1)
+    p.row = lambda i, pos: (int(p.table[0 if pos < prefix else i, pos // 20]), pos % 20)       # 2048 ends inside a page
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_prefix(cache, batch, q, out, p.scale, prefix)
+    assert "prefix" in nt.last_plan() and "x%d pieces=" % rows in nt.last_plan(), nt.last_plan()
+    assert_within(out, want, tol, nt.last_plan())
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_sequences_that_grow_past_a_prefix_in_a_replay(gpu, half):
+    """Recorded while all sequences end inside the prefix, replayed until all have it."""
+    import torch
+    p = Problem([300, 511, 20, 512, 480], [1] * 5, 8, 2, 64, 16, half, 91, prefix=512, uniform=True, slack=8, max_length=640)
+    own = torch.arange(40, dtype=torch.int32).view(5, 8)
+    p.table[:, 32:40] = p.k.shape[0] + own
+    more = [torch.randn((40, 16, 2, 64), generator=torch.Generator().manual_seed(i)).to(p.k.dtype) for i in (1, 2)]
+    p.k, p.v = torch.cat([p.k, more[0]]), torch.cat([p.v, more[1]])
+    for i in range(1, 5):                               # the reference goes by every sequence's own row
+        p.table[i, :32] = p.table[0, :32]
+    cache, batch, q, out = p.place(nt)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        nt.attention_prefix(cache, batch, q, out, p.scale, 512)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            nt.attention_prefix(cache, batch, q, out, p.scale, 512)
+    for lens in ([300, 511, 20, 512, 480], [400, 512, 0, 513, 511], [512, 600, 513, 639, 512], [1, 63, 64, 65, 640]):
+        p.lens = lens
+        p.lengths_d.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(77.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, tol = p.attention(True)
+        assert_within(out, want, tol, str(lens))
+
+
+# ---- pools and rows in other orders ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("order", ["keys and values side by side", "positions first", "heads first", "padded rows"])
+@pytest.mark.parametrize("new,page", [(1, 16), (40, 16), (40, 20), (40, 8), (40, 2)])
+def test_pools_in_any_order(gpu, half, order, new, page):
+    import torch
+    p = Problem([130, 64, 97], [new] * 3, 8, 2, 64, page, half, 92)
+    cache, batch, q, out = p.place(nt)
+    if order == "keys and values side by side":
+        both = torch.stack([p.k, p.v], 1).to(gpu)       # [pages][2][positions][heads][columns]
+        p.kd, p.vd = both[:, 0], both[:, 1]
+    elif order == "padded rows":
+        p.kd, p.vd = (torch.nn.functional.pad(x, (0, 8, 0, 1), value=float("nan")).to(gpu)[:, :, :2, :64] for x in (p.k, p.v))
+    else:
+        turn = (1, 0, 2, 3) if order == "positions first" else (2, 0, 1, 3)
+        back = [turn.index(i) for i in range(4)]
+        p.kd, p.vd = (x.permute(turn).contiguous().to(gpu).permute(back) for x in (p.k, p.v))
+    cache = nt.KVCache(p.kd, p.vd)
+    want, tol = p.attention(True)
+    nt.attention_cached(cache, batch, q, out, p.scale)
+    assert_within(out, want, tol, nt.last_plan())
+    k = torch.randn((p.tokens, 2, 64), device=gpu).to(q.dtype)
+    nt.cache_append(cache, batch, k, k)
+    for i in range(3):
+        for t in (0, new - 1):
+            page_, row = p.row(i, p.lens[i] - new + t)
+            assert torch.equal(p.kd[page_, row], k[p.starts[i] + t]) and torch.equal(p.vd[page_, row], k[p.starts[i] + t])
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_queries_and_rows_that_stand_for_many(gpu, new):
+    """Strides of zero: one query for all heads, one row of values for all tokens."""
+    import torch
+    p = Problem([130, 64], [new] * 2, 8, 2, 64, 16, True, 93)
+    p.q = p.q[:, :1].expand(-1, 8, -1).contiguous()
+    want, tol = p.attention(True)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_cached(cache, batch, q[:, :1].contiguous().expand(-1, 8, -1), out, p.scale)
+    assert_within(out, want, tol, nt.last_plan())
+    k, v = torch.randn((1, 1, 64), device=gpu).half().expand(p.tokens, 2, 64), torch.randn((1, 2, 64), device=gpu).half().expand(p.tokens, 2, 64)
+    nt.cache_append(cache, batch, k, v)
+    for i in range(2):
+        page, row = p.row(i, p.lens[i] - 1)
+        assert torch.equal(p.kd[page, row], k[0]) and torch.equal(p.vd[page, row], v[0])
+
+
 # ---- probabilities in half -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("new,heads,slack,split,plan", [
