@@ -425,9 +425,9 @@ def cache_append(cache, batch, k, v, rotation=None, pairs=False, q=None, q_out=N
     k0, k1, v0, v1, _ = _rows(k, v, cache, batch, cache.heads)
     q0 = q1 = o0 = o1 = heads = positions = rotated = 0
     qp = op = rp = None
+    if (q is None) != (q_out is None):
+        raise NtsAmdError("Unmatched tensors: queries need a [tokens][heads][dh] result, and the other way round")
     if q is not None:
-        if q_out is None:
-            raise NtsAmdError("Unmatched tensors: queries need a [tokens][heads][dh] result")
         q0, q1, o0, o1, heads = _rows(q, q_out, cache, batch)
         qp, op = q.data_ptr(), q_out.data_ptr()
     if rotation is not None:

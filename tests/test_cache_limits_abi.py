@@ -79,3 +79,12 @@ def test_numbers_beyond_32_bits_are_refused_by_the_binding():
     wide = torch.zeros(1, dtype=torch.float16).expand((1 << 32) + 3, 16, 2, 1)
     with pytest.raises(nt.NtsAmdError, match="32 bits"):
         nt.KVCache(wide, wide)
+
+
+def test_a_result_without_queries_is_refused_by_the_binding():
+    import torch
+    k = torch.zeros((4, 16, 2, 64), dtype=torch.float16)
+    batch = nt.CacheBatch(torch.ones(2, dtype=torch.int32), torch.zeros((2, 4), dtype=torch.int32))
+    new, q = torch.zeros((2, 2, 64), dtype=torch.float16), torch.zeros((2, 4, 64), dtype=torch.float16)
+    with pytest.raises(nt.NtsAmdError, match="queries"):
+        nt.cache_append(nt.KVCache(k, k.clone()), batch, new, new, q_out=q)
