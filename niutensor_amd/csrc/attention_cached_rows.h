@@ -23,8 +23,9 @@
  * The four waves' results meet in LDS. Where a range is not all of a sequence's keys, the result is a partial one
  * (unnormalised row, maximum, sum), and a second kernel joins them in the order of the keys.
  *
- * 64 sequences of up to 8191 positions, 32 heads on 8 of 128 columns, half: 201 us and 5 for the join, 5.3 TB/s; one of 131072: 95 and 5,
- * 5.6 TB/s. One of 128, 8 heads of 64: 4.1 us, of which the launch and four loads that each need the one before are nearly all.
+ * 64 sequences of up to 8191 positions, 32 heads on 8 of 128 columns, half: 202 us and 5 for the join, 5.3 TB/s; one of 131072: 95 and 5,
+ * 5.6 TB/s. One of 128, 8 heads of 64: 4.2 us replayed from a graph (a call through the host 5.3), of which the launch and four loads that
+ * each need the one before are nearly all.
  */
 #pragma once
 #include "gemm_common.h"

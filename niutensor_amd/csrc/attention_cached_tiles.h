@@ -1,7 +1,8 @@
 /*
  * Attention over a cache on pages for many query rows in half: pieces of text against what is in the cache, and the
- * queries of a whole batch against a prefix they share (ntsamd_attention_cached, ntsamd_attention_prefix; the few rows of a
- * decoding step and float go to attention_cached.hip).
+ * queries of a whole batch against a prefix they share (ntsamd_attention_cached, ntsamd_attention_prefix). The stages and the fetch are
+ * shared with float tiles of 64 rows (attention_cached_tiles_f32.h); the few rows of a decoding step, and tiles of 16 or 32 rows, are
+ * attention_cached_rows.h.
  *
  * Bound by the matrix instructions and what feeds them, so keys and values go through LDS once for all rows of a
  * workgroup, on the plan of attention_f16.hip: 64 QR rows (tokens x the query heads that share a key head) of a tile, 16 QR
@@ -16,8 +17,8 @@
  *
  * A wave's block of 64 keys, 32 rows and 128 columns is 1090 cycles of MFMAs and about as many of vector instructions, 512 of them
  * exponentials. 4 pieces of text of 257 to 1024 tokens in sequences of 1500 to 4096, 32 heads on 8 of 128: 121 us, 807 TFLOP/s with
- * the last round of workgroups half empty; 959 for 8 times 1024 on 4096 (837, 783, 529 with heads of 96, 64, 32; a large product
- * reaches 1207).
+ * the last round of workgroups half empty; 8 times 1024 on 4096, not causal: 592 us, 928 TFLOP/s (822, 753, 530 with heads of 96, 64, 32;
+ * a large product reaches 1207); causal 538 us, 894.
  */
 #pragma once
 #include "gemm_common.h"
@@ -30,7 +31,8 @@ namespace ntsamd {
 /* Two stages of a block of keys and values: KB keys, 32 KB at most, so that two workgroups share a CU. Rows are those of DHM columns,
    without padding (they are written 16 bytes a lane, one lane after the other); which 16-byte piece of a row stands where is
    swizzled by the row instead, so that 16 rows read at one column, and in half the pairs of pieces that a transposing read takes of
-   8 rows, spread over all banks. */
+   8 rows, stand on all banks once. That is so for lanes served in order; the counters still show conflicts, a third of the cycles
+   in which half tiles read LDS. */
 template <typename T, int DHM> struct CachedTilesShared {
     static constexpr int KB = cached_block_keys(sizeof(T) == 2, DHM, 64);
     static constexpr int PIECES = DHM * (int)sizeof(T) / 16, ROW = DHM * (int)sizeof(T), BLOCK = KB * ROW;

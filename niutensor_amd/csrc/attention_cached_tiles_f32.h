@@ -2,9 +2,11 @@
  * Float tiles of many rows of a sequence: the plan of attention_cached_tiles.h on the float matrix instruction, which takes
  * 32 cycles for 16 rows x 16 keys x 4 columns: bound by it, and softmax, LDS and the fetches hide behind it. (Tiles of 16 or 32
  * rows whose waves share the keys, attention_cached_rows.h, read a key row for each of them: 8 or 16 operations a byte, bound by
- * the caches when many run.) 512 tokens of 8 sequences to 2048 positions, 8 heads of 128: 295 us, 117 TFLOP/s (tiles of 32 rows 103, of 16
- * 82; a large product 146); of 96 columns 109 (85, 69), of 64 112 (93, 79), of 32 96 (79, 67); 8 times 1024 on 4096, 32 heads on 8 of 128: 123. The matrix unit is busy 81 % of a
- * wave's life there; the rest is the softmax and the barrier, which its one neighbour on the SIMD covers in part.
+ * the caches when many run.) 512 tokens of 8 sequences of 2048 positions, not causal, 8 heads of 128, in one piece: 295 us, 117 TFLOP/s
+ * (tiles of 32 rows 103, of 16 82; a large product 146); of 96 columns 109 (85, 69), of 64 112 (93, 79), of 32 96 (79, 67); 8 times 1024
+ * on 4096, 32 heads on 8 of 128: 122. (The plan's estimate takes the lengths of a batch for uneven: in these calls it takes tiles of 32
+ * rows with 128 columns, 329 us, and two pieces with fewer.) The matrix unit is busy 81 % of a wave's life there; the rest is the softmax
+ * and the barrier, which its one neighbour on the SIMD covers in part.
  *
  * S^T = K Q^T: lane (m, g) = (l % 16, l / 16) feeds columns 16 t + 4 g + e, e = 0..3, of key m and of query m, one 16-byte read for four
  * MFMAs. O^T = V^T P^T: it holds the probabilities of keys 4 g + r, feeds them as they are, and of V reads VC neighbouring columns,

@@ -3,10 +3,10 @@
  * sequences with the prefix, as tiles of one matrix, and workgroups that take each sequence's own keys. The first
  * wait on matrix instructions, the second on memory; taken in turn, eight of one kind and eight of the other (a workgroup
  * for each XCD), a CU has both. attention_join_kernel puts their partial results together.
- * 64 sequences of 8193 to 8704 positions behind a prefix of 8192, 8 key heads of 128, four query heads to each, half: 37 us and 7 us for
- * the join (28 us, 23 us and the join in launches of their own); the keys and values alone take 20 us at 5.1 TB/s. What is left is the
- * start of the workgroups, the blocks' first fetches, which nothing hides, and the partial results of the prefix's pieces (17 MB written
- * and read). Sequence by sequence, without the prefix read once, the same call takes 163 us.
+ * 64 sequences of 8193 to 8704 positions behind a prefix of 8192, 8 key heads of 128, four query heads to each, half: 36 us and 6 us for
+ * the join by the profiler, 41 us a call (28 us, 23 us and the join in launches of their own); the keys and values alone take 20 us at 5.1 TB/s.
+ * What is left is the start of the workgroups, the blocks' first fetches, which nothing hides, and the partial results of the prefix's
+ * pieces (17 MB written and read). Sequence by sequence, without the prefix read once, the same call takes 163 us.
  */
 #include "attention_cached_rows.h"
 #include "attention_cached_tiles.h"

@@ -12,8 +12,8 @@
  * and the row itself).
  * Rows that are not 16-byte aligned and numbers of turned columns that are no whole 16-byte pieces take items of one
  * column or pair instead.
- * 8 prompts of 513 to 2048 tokens, 32 heads on 8 of 128 columns, half: 46 us, 5.1 TB/s read and written; one token: 3.5 us, a launch and
- * the three loads; 64 sequences of one token: 3.5.
+ * 8 prompts of 513 to 2048 tokens, 32 heads on 8 of 128 columns, half: 45 us, 5.1 TB/s read and written. One token: 3.1 us, a launch and
+ * the three loads; 64 sequences of one token: 3.4; both replayed from a graph, calls of them one after the other take the host 6.
  */
 #include "gemm_common.h"
 #include "gemm_f16.h"       /* half_t */
@@ -179,7 +179,7 @@ bool deal_items(AppendParams & p)
         return false;
     p.items = (int)items;
     /* A lane's items follow one another, each a load and a store that wait for memory: one each where the waves run at once (64 sequences
-       of one token, 448 waves: 3.5 us; 4.6 with four). Beyond, what a wave does first counts, its look at the starts above all: two each
+       of one token, 448 waves, replayed: 3.5 us; 4.6 with four). Beyond, what a wave does first counts, its look at the starts above all: two each
        (1 to 499 tokens of 7 sequences, float: 9.3, 7.7, 8.4 us with one, two and four; 8 prompts 48.5, 45.7, 47.5), four with more
        than 64 sequences (87 of up to 108 tokens: 13.9, 11.8, 9.9). */
     const int looks = p.c.starts ? p.c.sequences / 64 + 1 : 1;
