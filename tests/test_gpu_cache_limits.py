@@ -128,6 +128,23 @@ def test_sequences_that_grow_past_a_prefix_in_a_replay(gpu, half):
         assert_within(out, want, tol, str(lens))
 
 
+# ---- batches of different sequences ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,new", [
+    ([2000, 1500, 17, 900, 1], [1, 1, 1, 200, 1]),      # steps of one token beside a piece of text
+    ([300, 2200, 64], [300, 2, 64]),                    # prompts, whose positions are all new, beside a step of two
+    ([513, 257, 128, 1], [513, 257, 128, 1]),           # prompts alone
+])
+def test_batches_of_different_sequences(gpu, half, causal, lens, new):
+    p = Problem(lens, new, 8, 2, 64, 16, half, 94, pad_tokens=1)
+    want, tol = p.attention(causal)
+    cache, batch, q, out = p.place(nt)
+    nt.attention_cached(cache, batch, q, out, p.scale, causal=causal)
+    assert_within(out, want, tol, nt.last_plan())
+
+
 # ---- pools and rows in other orders ------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("half", [True, False])
